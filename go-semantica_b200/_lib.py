@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(HERE, "libsemantica_b200.so")
 
 SEM_OK, SEM_EINVAL, SEM_EDEVICE, SEM_ENOMEM, SEM_EFORMAT, SEM_ENOTFOUND, SEM_EINTERNAL = range(7)
 SEARCH_REFERENCE, SEARCH_EXACT = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = range(3)
 
 
 class SemError(Exception):
@@ -77,6 +78,23 @@ _SIGNATURES = {
     "sem_q8_gemm_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "sem_q8_matmul_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "sem_q8_path": (C.c_int, [C.c_int32]),
+    "sem_adapter_plan_create": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.POINTER(C.c_void_p)]),
+    "sem_adapter_plan_set": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "sem_adapter_plan_free": (C.c_int, [C.c_void_p]),
+    "sem_lowrank_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_int32, C.POINTER(C.c_void_p)]),
+    "sem_lowrank_free": (C.c_int, [C.c_void_p]),
+    "sem_lowrank_apply": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64,
+                                    C.c_void_p, C.c_int32, C.c_int64, C.c_void_p]),
+    "sem_lowrank_apply_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
+                                         C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sem_lowrank_check": (C.c_int, [C.c_void_p]),
+    "sem_block_norm_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_int32,
+                                        C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "sem_block_norm_free": (C.c_int, [C.c_void_p]),
+    "sem_block_norm_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                     C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                     C.c_void_p]),
     "sem_index_build": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,
                                   C.POINTER(C.c_void_p)]),
     "sem_index_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "host/adapter_plan.h"
+
 namespace sem {
 
 // ---- load-time repacking (model_kernels.cu) ----
@@ -256,5 +258,87 @@ cudaError_t launch_split_int16(const void* src, int64_t rows, int dim, int src_r
 // rows of out_row_bytes (zero padded).
 cudaError_t launch_normalize_quantize(const float* in, int64_t count, int dim, int quant, int out_row_bytes,
                                       bool normalize, void* out, cudaStream_t stream);
+
+// ---- adapters of many requests (adapters.cu) ----
+// A batch's rows ordered by adapter, on the device (sem_adapter_plan): tiles
+// of positions that share an adapter, each position's row and sequence, each
+// row's adapter (-1: none). The kernels read the counts from `counts`, so a
+// captured launch follows a plan that is set again.
+struct AdapterPlanDev {
+  const int32_t* counts;       // [4] large tiles, small tiles, rows, sequences
+  const AdapterTile* large;    // up to kAdapterTileRows rows each
+  const AdapterTile* small;    // up to kAdapterSmallRows rows each
+  const int32_t* pos_row;      // [rows] the row at each position
+  const int32_t* pos_seq;      // [rows] and its sequence
+  const int32_t* row_adapter;  // [rows]
+};
+// pos_row, pos_seq and row_adapter from the sorted sequences: sequence i of
+// the order holds positions [pos[i], pos[i + 1]) and rows from row0[i] on.
+cudaError_t launch_adapter_plan(const int32_t* pos, const int32_t* row0, const int32_t* seq, const int32_t* adapter,
+                                int32_t n_seqs, int32_t rows, int32_t* pos_row, int32_t* pos_seq,
+                                int32_t* row_adapter, cudaStream_t stream);
+
+// Element types of the adapter operators (SEM_DTYPE_*).
+enum DType { kDtF32 = 0, kDtF16 = 1, kDtBF16 = 2 };
+constexpr int kLowRankMaxRank = 128;
+
+// One adapter of a bank: a [rank][ka] and b [n_out][rp] in the bank's type,
+// 16-byte aligned rows, zeros in columns [k_in, ka) and [rank, rp).
+struct LowRankAdapter {
+  const void* a;
+  const void* b;
+  int32_t rank, rp;
+  float scale;
+};
+struct LowRankBank {
+  const LowRankAdapter* adapters;  // [n_adapters] on the device
+  int32_t n_adapters, k_in, n_out, ka;
+  int32_t wtype;     // DType of the weights
+  int32_t max_rank;
+};
+// y[row] = base[row] + scale * (x[row] * xs) A^T B^T of the row's adapter (rows
+// without one, or whose adapter has rank 0: y = base). base may be y or null
+// (zeros). Row strides in elements. absmax (nullable): x holds INT8 codes as
+// fp16 and xs = absmax[seq or 0] / 127 (seq when per_seq), otherwise xs = 1.
+struct LowRankArgs {
+  const void* x;
+  const void* base;
+  void* y;
+  int64_t ldx, ldb, ldy;
+  int32_t xtype, ytype;  // (f32, f32), (f16 | bf16, the same or f32)
+  const uint32_t* absmax;
+  int32_t per_seq;
+};
+// `tiles` of the plan on CUDA cores (any rows per tile; a cluster of CTAs each).
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, bool large_tiles, int n_tiles,
+                                 const LowRankArgs& args, cudaStream_t stream);
+
+// h_out = scale * h + gate * (rmsnorm(o) * post), y = rmsnorm(h_out before its
+// rounding) * pre: gate and scale of the row's adapter (adapter 0 for every
+// row when row_adapter is null; rows without one: 1). post null: o as it is;
+// pre null: no y. o and y in `dtype`, h and h_out in `htype` (dtype or f32).
+// h_out may be h and y may be o. absmax (nullable): atomic max of |y| into
+// absmax[row_seq[row]].
+constexpr int kBlockNormMaxDim = 16384;
+struct BlockNormArgs {
+  const void* o;
+  const void* h;
+  void* h_out;
+  void* y;
+  int64_t ldo, ldh, ldho, ldy;
+  int32_t dtype, htype;
+  int64_t rows;
+  int32_t dim;
+  float eps;
+  const float* post;
+  const float* pre;
+  const float* gates;   // [n_adapters][dim], null: 1
+  const float* scales;  // [n_adapters], null: 1
+  int32_t n_adapters;
+  const int32_t* row_adapter;
+  const int32_t* row_seq;
+  uint32_t* absmax;
+};
+cudaError_t launch_block_norm(const BlockNormArgs& args, cudaStream_t stream);
 
 }  // namespace sem

@@ -39,6 +39,9 @@ typedef struct sem_model sem_model;
 typedef struct sem_index sem_index;
 typedef struct sem_q8_weight sem_q8_weight;
 typedef struct sem_group sem_group;
+typedef struct sem_adapter_plan sem_adapter_plan;
+typedef struct sem_lowrank sem_lowrank;
+typedef struct sem_block_norm sem_block_norm;
 
 /* Message of the last failed call on this thread (never NULL). A Go caller
  * holds its OS thread (runtime.LockOSThread) from the failing call until it
@@ -283,6 +286,94 @@ int sem_q8_path(int32_t mode);
  * streams, other threads) race on it. Enqueued on `stream` (NULL = the
  * weight's context stream). */
 int sem_q8_gemm_noalloc(sem_q8_weight *w, const float *d_a, int32_t m, float *d_c, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Adapters of many requests beside one shared base model. No counterpart in
+ * the reference, which serves one model without adapters. A batch is packed
+ * sequences, as for sem_embed; each sequence names an adapter or none. The
+ * plan says which adapter every row uses; the operators below go by it. A
+ * plan, a bank and a block norm belong to one device; the calls take device
+ * pointers, are enqueued on `stream` (NULL = the handle's context stream) and
+ * return without synchronising. They allocate nothing and keep no state, so
+ * calls may overlap, on one stream or several, and may be captured into CUDA
+ * graphs.
+ * ---------------------------------------------------------------------- */
+
+/* Element types of the operators' rows and weights. */
+#define SEM_DTYPE_F32 0
+#define SEM_DTYPE_F16 1
+#define SEM_DTYPE_BF16 2
+
+/* A plan for batches of up to max_rows rows in up to max_seqs sequences. */
+int sem_adapter_plan_create(sem_context *ctx, int64_t max_rows, int32_t max_seqs, sem_adapter_plan **out);
+/* Sets the batch (host arrays, copied): sequence s is rows
+ * [offsets[s], offsets[s+1]) (offsets[0] = 0, empty sequences allowed) and
+ * uses adapters[s], -1 for none; several sequences may use one adapter. The
+ * tables are uploaded on `stream`: work that uses the plan is ordered after
+ * the call there, and work enqueued earlier that still reads the plan's
+ * previous batch must be on the same stream or done. Not inside a stream
+ * capture; a captured operator reads the batch that the plan holds when the
+ * graph is replayed (a plan set to another batch needs no new capture; the
+ * caller keeps its buffers as large as that batch needs, and its adapter
+ * indexes within the bank: a row of an adapter that the bank does not have is
+ * then treated as a row without one). */
+int sem_adapter_plan_set(sem_adapter_plan *plan, const int32_t *offsets, const int32_t *adapters, int32_t n_seqs,
+                         void *stream);
+int sem_adapter_plan_free(sem_adapter_plan *plan);
+
+/* Low-rank adapters of one projection (k_in -> n_out, each 1..65536): adapter
+ * i has weights a[i] [ranks[i]][k_in] and b[i] [n_out][ranks[i]] (host
+ * pointers, row-major, of element type dtype, copied) and the factor
+ * scales[i]; ranks 0..128, 0 for an adapter that leaves this projection as it
+ * is (its pointers are not read). */
+int sem_lowrank_create(sem_context *ctx, int32_t k_in, int32_t n_out, int32_t n_adapters, const int32_t *ranks,
+                       const float *scales, const void *const *a, const void *const *b, int32_t dtype,
+                       sem_lowrank **out);
+int sem_lowrank_free(sem_lowrank *w);
+/* For every row of the plan's batch, with its sequence's adapter i:
+ *   y = base + scales[i] * (x a[i]^T) b[i]^T,
+ * and y = base for rows without an adapter. x: k_in values a row; base and y:
+ * n_out values a row of y's type, base is normally the shared projection's
+ * output (sem_q8_gemm). base may be y itself, or NULL for zeros; apart from
+ * that y overlaps neither x nor base. Row strides ldx, ld_base, ldy in
+ * elements, 0 for packed rows; any stride and any element-aligned address is
+ * allowed (rows that start on 16 bytes load fastest). Types: x F32 with y
+ * F32; x F16 or BF16 with y of the same type or F32. Products and sums are
+ * held in float32, with x, the weights and the rank-wide intermediate carried
+ * to at least 21 bits; the result is rounded once, to y's type. */
+int sem_lowrank_apply(sem_lowrank *w, sem_adapter_plan *plan, const void *d_x, int32_t x_dtype, int64_t ldx,
+                      const void *d_base, int64_t ld_base, void *d_y, int32_t y_dtype, int64_t ldy, void *stream);
+/* The same beside sem_q8_matmul_int8: x = code * (absmax / 127), d_codes the
+ * rows x k_in INT8 codes as fp16, d_absmax the float32 bit patterns of the
+ * absmax they were quantised with: one for every row (n_absmax = 1), or one
+ * per sequence of the plan (n_absmax = n_seqs). */
+int sem_lowrank_apply_int8(sem_lowrank *w, sem_adapter_plan *plan, const void *d_codes, const uint32_t *d_absmax,
+                           int32_t n_absmax, const float *d_base, int64_t ld_base, float *d_y, int64_t ldy,
+                           void *stream);
+/* Waits for the device and reports what its calls recorded since the last
+ * check: SEM_EDEVICE when a tensor-core pipeline wait timed out (that call's
+ * output is incomplete). */
+int sem_lowrank_check(sem_lowrank *w);
+
+/* The norms after a block and before the next one, fused with the block's
+ * gate and residual scale (host pointers, copied): post_w, pre_w [dim] (NULL:
+ * that norm is left out), gates [n_adapters][dim] (NULL: 1), scales
+ * [n_adapters] (NULL: 1), dim 1..16384. */
+int sem_block_norm_create(sem_context *ctx, int32_t dim, float eps, const float *post_w, const float *pre_w,
+                          int32_t n_adapters, const float *gates, const float *scales, sem_block_norm **out);
+int sem_block_norm_free(sem_block_norm *b);
+/* For every row, with its adapter i (plan NULL: i = 0 for every row; rows
+ * without an adapter: gate and scale 1):
+ *   h_out = scales[i] * h + gates[i] * (rmsnorm(o) * post_w)
+ *   y     = rmsnorm(h_out) * pre_w        (from h_out before its rounding)
+ * rmsnorm(v) = v / sqrt(mean(v^2) + eps), in float32; o itself without
+ * post_w, no y (d_y is not used) without pre_w. o and y are of type dtype, h
+ * and h_out of type h_dtype (dtype, or F32). h_out may be h, y may be o; no
+ * other overlap. `rows` is the plan's row count when there is a plan. Strides
+ * as for sem_lowrank_apply. */
+int sem_block_norm_run(sem_block_norm *b, sem_adapter_plan *plan, int64_t rows, const void *d_o, int64_t ldo,
+                       int32_t dtype, const void *d_h, int64_t ldh, int32_t h_dtype, void *d_h_out, int64_t ld_h_out,
+                       void *d_y, int64_t ldy, void *stream);
 
 /* ------------------------------------------------------------------------
  * Brute-force index: replaces search/brute (builder.go, index.go, storage.go).
