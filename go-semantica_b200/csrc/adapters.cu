@@ -96,7 +96,7 @@ constexpr int kSmallChunk = 128;  // input channels staged at a time, 4 per lane
 
 template <class XT, class YT>
 __global__ void __cluster_dims__(kSmallCtas, 1, 1) __launch_bounds__(kSmallThreads)
-    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, int large_tiles, LowRankArgs a) {
+    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, LowRankArgs a) {
   constexpr int R = kAdapterSmallRows;
   __shared__ __align__(16) float s_x[R][kSmallChunk];
   __shared__ __align__(16) float s_part[kLowRankMaxRank][R];
@@ -106,8 +106,7 @@ __global__ void __cluster_dims__(kSmallCtas, 1, 1) __launch_bounds__(kSmallThrea
   cg::cluster_group cluster = cg::this_cluster();
   const int rank_id = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const AdapterTile* tiles = large_tiles ? plan.large : plan.small;
-  const int n_tiles = plan.counts[large_tiles ? 0 : 1];
+  const int n_tiles = plan.counts[1];
   const XT* x = static_cast<const XT*>(a.x);
   const YT* base = static_cast<const YT*>(a.base);
   YT* y = static_cast<YT*>(a.y);
@@ -118,8 +117,8 @@ __global__ void __cluster_dims__(kSmallCtas, 1, 1) __launch_bounds__(kSmallThrea
   const int n0 = min(bank.n_out, rank_id * nper), n1 = min(bank.n_out, n0 + nper);
 
   for (int tile = (int)(blockIdx.x / kSmallCtas); tile < n_tiles; tile += (int)(gridDim.x / kSmallCtas)) {
-    const AdapterTile tl = tiles[tile];
-    LowRankAdapter ad{nullptr, nullptr, 0, 0, 0.0f};
+    const AdapterTile tl = plan.small[tile];
+    LowRankAdapter ad{};
     if (tl.adapter >= 0 && tl.adapter < bank.n_adapters) ad = bank.adapters[tl.adapter];
     if (ad.rank == 0 && a.base == a.y && a.ldb == a.ldy) continue;  // in place and nothing to add (the whole cluster)
     for (int sub = 0; sub < tl.rows; sub += R) {
@@ -368,10 +367,10 @@ cudaError_t norm_types(const BlockNormArgs& a, cudaStream_t st) {
 }
 
 template <class XT, class YT>
-cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, bool large, int n_tiles,
-                        const LowRankArgs& a, cudaStream_t st) {
+cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles, const LowRankArgs& a,
+                        cudaStream_t st) {
   const int clusters = n_tiles < 4096 ? n_tiles : 4096;
-  lowrank_small_kernel<XT, YT><<<clusters * kSmallCtas, kSmallThreads, 0, st>>>(bank, plan, large ? 1 : 0, a);
+  lowrank_small_kernel<XT, YT><<<clusters * kSmallCtas, kSmallThreads, 0, st>>>(bank, plan, a);
   return cudaGetLastError();
 }
 
@@ -386,18 +385,18 @@ cudaError_t launch_adapter_plan(const int32_t* pos, const int32_t* row0, const i
   return cudaGetLastError();
 }
 
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, bool large_tiles, int n_tiles,
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
                                  const LowRankArgs& a, cudaStream_t st) {
   if (n_tiles <= 0) return cudaSuccess;
-  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, large_tiles, n_tiles, a, st);
+  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, n_tiles, a, st);
   if (a.xtype == kDtF16 && a.ytype == kDtF16)
-    return small_types<__half, __half>(bank, plan, large_tiles, n_tiles, a, st);
+    return small_types<__half, __half>(bank, plan, n_tiles, a, st);
   if (a.xtype == kDtF16 && a.ytype == kDtF32)
-    return small_types<__half, float>(bank, plan, large_tiles, n_tiles, a, st);
+    return small_types<__half, float>(bank, plan, n_tiles, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtBF16)
-    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, large_tiles, n_tiles, a, st);
+    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, n_tiles, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtF32)
-    return small_types<__nv_bfloat16, float>(bank, plan, large_tiles, n_tiles, a, st);
+    return small_types<__nv_bfloat16, float>(bank, plan, n_tiles, a, st);
   return cudaErrorInvalidValue;
 }
 

@@ -11,7 +11,7 @@ namespace sem {
 
 // Rows of a large tile, and the most rows of a small one (the kernels of
 // kernels.h, launch_lowrank_*).
-constexpr int kAdapterTileRows = 128;
+constexpr int kAdapterTileRows = 64;
 constexpr int kAdapterSmallRows = 16;
 
 // Up to kAdapterTileRows positions [pos0, pos0 + rows) of the order by adapter

@@ -138,10 +138,10 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
   std::unique_ptr<sem_lowrank> w(new sem_lowrank());
   w->ctx = ctx;
   const size_t es = dtype_size(dtype);
-  const int32_t ka = (int32_t)round_up(k_in, 32);
+  const int32_t ka = (int32_t)round_up(k_in, 64);
   // host image: the adapter table, then every adapter's a and b, rows padded with zeros
   size_t bytes = (size_t)round_up((int64_t)n_adapters * sizeof(LowRankAdapter), 256);
-  std::vector<size_t> at_a(n_adapters), at_b(n_adapters);
+  std::vector<size_t> at_a(n_adapters), at_b(n_adapters), at_ta(n_adapters), at_tb(n_adapters);
   int32_t max_rank = 0;
   for (int32_t i = 0; i < n_adapters; ++i) {
     const int64_t rp = round_up(ranks[i], 8);
@@ -151,13 +151,21 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
     bytes += (size_t)round_up((int64_t)n_out * rp * es, 256);
     if (ranks[i] > max_rank) max_rank = ranks[i];
   }
-  if (bytes == 0) bytes = 256;
-  cudaError_t e = w->weights.ensure(bytes);
+  // behind the image, filled on the device: the weights as the tensor-core kernel's tiles
+  size_t total = bytes;
+  for (int32_t i = 0; i < n_adapters; ++i) {
+    at_ta[i] = total;
+    total += lowrank_tile_bytes_a(ranks[i], ka, dtype);  // multiples of 128 bytes
+    at_tb[i] = total;
+    total += lowrank_tile_bytes_b((int)round_up(ranks[i], 8), n_out, dtype);
+  }
+  cudaError_t e = w->weights.ensure(total > 0 ? total : 256);
   if (e != cudaSuccess)
-    return set_error(SEM_ENOMEM, "device allocation of %zu bytes failed: %s", bytes, cudaGetErrorString(e));
+    return set_error(SEM_ENOMEM, "device allocation of %zu bytes failed: %s", total, cudaGetErrorString(e));
   e = w->err.ensure(16);
   if (e != cudaSuccess) return set_error(SEM_ENOMEM, "device allocation failed: %s", cudaGetErrorString(e));
   std::vector<uint8_t> img(bytes, 0);
+  std::vector<LowRankAdapter> table(n_adapters);
   uint8_t* d = w->weights.as<uint8_t>();
   for (int32_t i = 0; i < n_adapters; ++i) {
     const int32_t r = ranks[i], rp = (int32_t)round_up(r, 8);
@@ -167,11 +175,13 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
     for (int32_t n = 0; r > 0 && n < n_out; ++n)
       std::memcpy(&img[at_b[i] + (size_t)n * rp * es], static_cast<const uint8_t*>(b[i]) + (size_t)n * r * es,
                   (size_t)r * es);
-    const LowRankAdapter ad{d + at_a[i], d + at_b[i], r, rp, scales[i]};
+    const LowRankAdapter ad{d + at_a[i], d + at_b[i], d + at_ta[i], d + at_tb[i], r, rp, scales[i]};
+    table[i] = ad;
     std::memcpy(&img[(size_t)i * sizeof(LowRankAdapter)], &ad, sizeof ad);
   }
   std::lock_guard<std::mutex> lk(ctx->mu);
-  SEM_CUDA(cudaMemcpyAsync(d, img.data(), bytes, cudaMemcpyHostToDevice, ctx->stream));
+  if (bytes) SEM_CUDA(cudaMemcpyAsync(d, img.data(), bytes, cudaMemcpyHostToDevice, ctx->stream));
+  for (const LowRankAdapter& ad : table) SEM_CUDA(launch_lowrank_tiles(ad, k_in, n_out, ka, dtype, ctx->stream));
   SEM_CUDA(cudaMemsetAsync(w->err.p, 0, 16, ctx->stream));
   SEM_CUDA(cudaStreamSynchronize(ctx->stream));
   w->bank = LowRankBank{reinterpret_cast<const LowRankAdapter*>(d), n_adapters, k_in, n_out, ka, dtype, max_rank};
@@ -201,12 +211,11 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, const LowRankArgs& ar
 // set to another batch, so a capture records a launch for each list.
 int lowrank_enqueue(const LowRankBank& bank, const sem_adapter_plan* plan, const LowRankArgs& args, bool captured,
                     uint32_t* err, cudaStream_t st) {
-  (void)err;
   const AdapterPlanDev dev = plan_device(plan);
   if (plan->n_large > 0 || captured)
-    SEM_CUDA(launch_lowrank_small(bank, dev, true, plan->n_large > 0 ? plan->n_large : 1, args, st));
+    SEM_CUDA(launch_lowrank_tc(bank, dev, plan->n_large > 0 ? plan->n_large : 1, args, err, st));
   if (plan->n_small > 0 || captured)
-    SEM_CUDA(launch_lowrank_small(bank, dev, false, plan->n_small > 0 ? plan->n_small : 1, args, st));
+    SEM_CUDA(launch_lowrank_small(bank, dev, plan->n_small > 0 ? plan->n_small : 1, args, st));
   return SEM_OK;
 }
 

@@ -287,6 +287,8 @@ constexpr int kLowRankMaxRank = 128;
 struct LowRankAdapter {
   const void* a;
   const void* b;
+  const uint8_t* ta;  // a and b as the tensor-core kernel's tiles (launch_lowrank_tiles)
+  const uint8_t* tb;
   int32_t rank, rp;
   float scale;
 };
@@ -309,9 +311,19 @@ struct LowRankArgs {
   const uint32_t* absmax;
   int32_t per_seq;
 };
-// `tiles` of the plan on CUDA cores (any rows per tile; a cluster of CTAs each).
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, bool large_tiles, int n_tiles,
+// The plan's small tiles on CUDA cores (adapters.cu).
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
                                  const LowRankArgs& args, cudaStream_t stream);
+
+// The large tiles on the tensor cores (lowrank_tc.cu). `err` (nullable)
+// receives error bits if a pipeline wait times out.
+cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
+                              const LowRankArgs& args, uint32_t* err, cudaStream_t stream);
+// Bytes of an adapter's ta and tb, and the kernel that fills them from a and b.
+size_t lowrank_tile_bytes_a(int rank, int ka, int wtype);
+size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype);
+cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, int ka, int wtype,
+                                 cudaStream_t stream);
 
 // h_out = scale * h + gate * (rmsnorm(o) * post), y = rmsnorm(h_out before its
 // rounding) * pre: gate and scale of the row's adapter (adapter 0 for every

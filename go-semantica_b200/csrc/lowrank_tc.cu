@@ -1,0 +1,859 @@
+// Low-rank adapters of large tiles on the sm_100a tensor cores.
+//
+//   y[row] = base[row] + s (x[row] A^T) B^T
+//
+// A unit is up to RT rows of one adapter (and a share of the output channels
+// when there are few rows). The shrink t = x A^T has the rows on the M lanes
+// and the ranks on N; the expand D = B t^T has output channels on the lanes
+// and the rows on N, so that the epilogue's threads read base and write y
+// along the channels of a row, coalesced. Two expand accumulators hold the
+// even and the odd channels of 256: a thread owns two neighbours.
+//
+// Numbers. The operands are tf32 (11 significant bits): fp16, bf16 and INT8
+// codes are exact in it; a float32 value v goes in as two parts, hi = v cut to
+// 11 bits and lo = v - hi (exact, of which the tensor core keeps 11 bits), and
+// hi hi + hi lo + lo hi are accumulated in float32 in TMEM, so products keep at
+// least 21 bits. t stays float32 between the products (hi and lo again). Only
+// y's own rounding loses bits.
+//
+// Bound by HBM at the ranks in use: a row moves k |x| + 2 n |y| bytes and
+// needs 2 r (k + n) flops (r = 16, 768 x 768, float32: 9.2 KB against 49
+// kflop, two products each: 0.02 of the tensor pipe). So the work is to keep
+// loads in flight and every other role short:
+//   - X warps (8): rows of x through registers (32 KB in flight, any row order
+//     and alignment), split and stored 128-byte swizzled;
+//   - two copy threads: the adapter's A and B tiles, which the bank keeps as
+//     tf32 planes in the swizzled layout, with one bulk copy per plane;
+//   - a shrink and an expand MMA thread, so that the shrink of later units
+//     goes on while the epilogue holds up the expand of an earlier one;
+//   - T warps (2): t from TMEM, scaled, split, to shared memory;
+//   - epilogue warps (8): base prefetched ahead of the accumulators.
+// One persistent CTA per SM.
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "sm100.cuh"
+
+namespace sem {
+
+namespace {
+
+constexpr int kXWarps = 8, kEpiWarps = 8, kTWarps = 2;
+constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
+constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1;
+constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA and copy warps, two idle
+// Registers: 768 threads get 80 each at launch; the last two warpgroups give
+// 32 back (256 x 48), the epilogue's take them (256 x 112).
+static_assert(kWarpB < kThreads / 32 && 256 * 80 + 256 * 112 + 256 * 48 <= kThreads * 80, "register split");
+static_assert(kWarpEpi % 4 == 0 && kWarpT % 4 == 0, "TMEM lane quarters go by warp index");
+constexpr int KC = 32;   // tf32 per swizzled 128-byte row
+constexpr int KS = 64;   // input channels per stage: two such rows
+constexpr int kRt = 64;  // rows per unit at most
+static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile or a part of one");
+constexpr int kMaxSlots = 4;
+constexpr int kXAhead = 2;  // stages of x prefetched to L2 ahead of the loads
+constexpr int kBPlane = 128 * 128;  // one plane of a slot of B: 128 channels x 128 bytes
+constexpr int kMiscBytes = 512 + kEpiWarps * 32 * 4;
+constexpr int kMaxSmem = 232448;  // an MMA reads 128 rows from a slot's start: a short slot's run on into sW and sT
+
+__device__ uint32_t g_lowrank_error;
+
+// kind::tf32, both operands K-major, float32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) {
+  return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// One lane of a converged warp. Unlike a test of the lane number it tells the
+// compiler that a single thread goes on, which the operands of an MMA need: 30
+// instead of 110 cycles to issue one.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The low word of a K-major 128-byte-swizzled operand's descriptor at shared
+// address `a`; its high word is the same for all. One thread issues every MMA,
+// so its instructions per MMA set their rate: moving 32 bytes (one K step)
+// along a row is + 2 on the low word.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t a) { return ((a & 0x3FFFFu) >> 4) | 1u << 16; }
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint64_t desc_at(uint32_t lo) { return pack2u(lo, kDescHi); }
+
+// A position in a ring of slots: the slot and the parity of its use.
+struct Ring {
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void next(uint32_t slots) {
+    if (++slot == slots) slot = 0, parity ^= 1;
+  }
+};
+
+// Contiguous copy global -> shared, completing as transaction bytes on bar.
+// Both addresses and the size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// mbar_wait's contract (bounded, gives up when another thread has) for short
+// stages: the clock is the SM's own and read only once a wait is long, since
+// reading the global timer takes longer than most of these waits.
+constexpr long long kWaitCycles = 4000000000ll;  // 2 s at 2 GHz
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* err,
+                                           uint32_t code) {
+  const uint32_t a = smem_u32(bar);
+  long long t0 = 0;
+  for (uint32_t n = 1; !mbar_try_wait(a, parity); ++n) {
+    if (n & 255) continue;
+    if (*abort_flag) return false;
+    const long long t = clock64();
+    if (!t0) t0 = t;
+    if (t - t0 > kWaitCycles) {
+      *abort_flag = 1;
+      atomicOr(err, code);
+      return false;
+    }
+  }
+  return true;
+}
+
+// A whole warp's wait: the same answer in every lane (each lane's own wait is
+// bounded), so that a warp leaves its loop as one.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* err,
+                                          uint32_t code) {
+  return __all_sync(0xffffffffu, stage_wait(bar, parity, abort_flag, err, code));
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// v = hi + lo: hi the upper 11 significant bits. |lo| < 2^-11 * 2^128 < 2e35,
+// so the maximum only replaces the NaN that an infinite v leaves in lo (which
+// would turn an infinite result into NaN); a NaN v stays one in hi.
+__device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
+  hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+  lo = fmaxf(__fsub_rn(v, hi), -2e35f);
+}
+
+template <class T>
+__device__ __forceinline__ float as_f32(T v) {
+  if constexpr (std::is_same<T, float>::value) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <class T>
+__device__ __forceinline__ T as_type(float v) {
+  if constexpr (std::is_same<T, float>::value) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+
+// 32 lanes x 8 columns of TMEM.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void reg_barrier8(uint32_t (&r)[8]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
+__device__ __forceinline__ void reg_barriern(uint32_t (&r)[16]) { reg_barrier16(r); }
+__device__ __forceinline__ void reg_barriern(uint32_t (&r)[8]) { reg_barrier8(r); }
+
+// The 256 TMEM columns of t's accumulators. The tensor core cuts every sum it
+// forms, an error that grows with the number of sums into one accumulator and
+// with its size; so the products run into up to four accumulators (the low
+// parts into one of their own, the stages of k over the others), which the T
+// warps add with rounding. Banks of ranks up to 64 have two sets in turn.
+struct ShrinkAcc {
+  int bufs, width, hi_parts, parts;
+  __device__ __forceinline__ ShrinkAcc(int max_rank, int rank, bool low, int k_stages) {
+    bufs = max_rank <= 64 ? 2 : 1;
+    width = (rank + 15) & ~15;  // N of the product: a multiple of 16
+    parts = min(4, 256 / bufs / width);
+    hi_parts = min(low ? parts - 1 : parts, k_stages);
+    parts = hi_parts + (low ? 1 : 0);
+  }
+};
+
+struct Unit {
+  LowRankAdapter ad;
+  int32_t pos0, rows;  // positions; rows <= 0: nothing
+  int32_t c0, c1;      // chunks of 256 output channels
+};
+
+struct TcParams {
+  LowRankBank bank;
+  AdapterPlanDev plan;
+  LowRankArgs a;
+  int32_t rt, splits;        // rows per unit (16, 32 or 64), shares of the output channels
+  int32_t x_slots, a_slots, b_slots, t_bufs;  // ring depths
+  int32_t x_vec;  // rows of x start on 16 bytes
+  int32_t y_vec;  // channels of base and y can be accessed in pairs
+  uint32_t* err;
+};
+
+// Unit u: sub-tiles of the same number lie together, so that those behind a
+// tile's last row (they are skipped) come last.
+__device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t u) {
+  Unit r;
+  const int split = (int)(u % p.splits);
+  const int64_t v = u / p.splits;
+  const AdapterTile tl = p.plan.large[v % n_tiles];
+  const int off = (int)(v / n_tiles) * p.rt;
+  r.pos0 = tl.pos0 + off;
+  r.rows = min(p.rt, tl.rows - off);
+  const int chunks = (p.bank.n_out + 255) / 256;
+  r.c0 = chunks * split / p.splits;
+  r.c1 = chunks * (split + 1) / p.splits;
+  r.ad = LowRankAdapter{};
+  if (r.rows > 0 && r.c1 > r.c0 && tl.adapter >= 0 && tl.adapter < p.bank.n_adapters)
+    r.ad = p.bank.adapters[tl.adapter];
+  return r;
+}
+
+// One chunk of a warp: rows [i0, i1) of the unit, channels ch and ch + 1 of
+// each lane, whose accumulators are the columns at `acc` (even channels) and
+// rt further (odd). `wait` (the accumulators are complete) is called between
+// the first loads of base and their use. VEC 2: the pair is accessed as one.
+template <class YT, int VEC, class Wait>
+__device__ __forceinline__ void epilogue_rows(const YT* base, YT* y, const int32_t* rows, int64_t ldb, int64_t ldy,
+                                              int ch, int n_out, int i0, int i1, uint32_t acc, int rt, Wait wait) {
+  struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
+  constexpr int B = VEC == 2 ? 16 : 8;
+  // Loads without conditions (rows behind the last one repeat it, channels behind n_out read the last ones), held in
+  // their own type: a condition or a conversion in between would make each load wait for the one before.
+  const int c0 = VEC == 2 ? min(ch, n_out - 2) : min(ch, n_out - 1), c1 = min(ch + 1, n_out - 1);
+  Pair nxt[B];
+  auto fetch = [&](int i) {
+    if (base) {
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const YT* b = base + (int64_t)rows[i - i0 + j] * ldb;
+        if (VEC == 2) nxt[j] = *reinterpret_cast<const Pair*>(b + c0);
+        else nxt[j].e[0] = b[c0], nxt[j].e[1] = b[c1];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < B; ++j) nxt[j].e[0] = nxt[j].e[1] = as_type<YT>(0.0f);
+    }
+  };
+  if (i0 < i1) fetch(i0);
+  if (!wait()) return;
+  for (int i = i0; i < i1; i += B) {
+    uint32_t v0[B], v1[B];
+    tmem_ldn(acc + (uint32_t)i, v0);
+    tmem_ldn(acc + (uint32_t)(rt + i), v1);
+    tmem_wait_ld();
+    reg_barriern(v0);
+    reg_barriern(v1);
+    Pair out[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      out[j].e[0] = as_type<YT>(__fadd_rn(as_f32(nxt[j].e[0]), __uint_as_float(v0[j])));
+      out[j].e[1] = as_type<YT>(__fadd_rn(as_f32(nxt[j].e[1]), __uint_as_float(v1[j])));
+    }
+    if (i + B < i1) fetch(i + B);
+    const int live = i1 - i;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (j >= live) break;
+      YT* d = y + (int64_t)rows[i - i0 + j] * ldy + ch;
+      if (VEC == 2) {
+        if (ch < n_out) *reinterpret_cast<Pair*>(d) = out[j];
+      } else {
+        if (ch < n_out) d[0] = out[j].e[0];
+        if (ch + 1 < n_out) d[1] = out[j].e[1];
+      }
+    }
+  }
+}
+
+template <class XT, class YT>
+__global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_constant__ TcParams p) {
+  constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;  // planes of x
+  constexpr int XE = 16 / sizeof(XT);                         // elements of one 16-byte load
+  constexpr int XL = KS / XE;                                 // loads per row and stage
+  constexpr int XR = kXWarps * 32 / XL;                       // rows per pass of the X warps
+  constexpr int XV = kRt / XR;                                // passes
+  constexpr int XD = 8 / XV;                                  // stages in flight: 8 loads per thread, 32 KB per SM
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int PW = p.bank.wtype == kDtF32 ? 2 : 1;  // planes of the weights
+  const int x_atom = p.rt * 128, x_slot = PX * 2 * x_atom;  // [plane][32 channels][rt rows][128 B]
+  const int a_rows = (p.bank.max_rank + 15) & ~15, a_slot = PW * 2 * a_rows * 128, b_slot = PW * kBPlane;
+  const int t_plane = p.rt * 128, t_chunks = (p.bank.max_rank + KC - 1) / KC;  // [chunk][hi, lo][rt rows][128 B]
+  uint8_t* sX = smem;
+  uint8_t* sA = sX + p.x_slots * x_slot;
+  uint8_t* sB = sA + p.a_slots * a_slot;
+  uint8_t* sT = sB + p.b_slots * b_slot;
+  const int t_buf = t_chunks * 2 * t_plane;
+  uint8_t* misc = sT + p.t_bufs * t_buf;
+  uint64_t* xfull = reinterpret_cast<uint64_t*>(misc);
+  uint64_t* xempty = xfull + kMaxSlots;
+  uint64_t* afull = xempty + kMaxSlots;   // weights of the shrink and of the expand
+  uint64_t* aempty = afull + kMaxSlots;
+  uint64_t* bfull = aempty + kMaxSlots;
+  uint64_t* bempty = bfull + kMaxSlots;
+  uint64_t* tafull = bempty + kMaxSlots;  // a shrink accumulator is complete / read
+  uint64_t* taempty = tafull + 2;
+  uint64_t* tfull = taempty + 2;          // t in shared memory is written / free
+  uint64_t* tfree = tfull + 2;
+  uint64_t* dfull = tfree + 2;            // an expand accumulator is complete / read
+  uint64_t* dempty = dfull + 2;
+  uint64_t* drain = dempty + 2;           // [2] the MMA threads' last MMAs
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
+  int32_t* s_row = reinterpret_cast<int32_t*>(misc + 512);      // [epilogue warp][64] rows of its half of the unit
+  uint32_t* err = p.err ? p.err : &g_lowrank_error;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMaxSlots; ++i) {
+      mbar_init(&xfull[i], kXWarps);
+      mbar_init(&xempty[i], 1);
+      mbar_init(&afull[i], 1);
+      mbar_init(&aempty[i], 1);
+      mbar_init(&bfull[i], 1);
+      mbar_init(&bempty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tafull[i], 1);
+      mbar_init(&taempty[i], kTWarps);
+      mbar_init(&dfull[i], 1);
+      mbar_init(&dempty[i], kEpiWarps);
+      mbar_init(&tfull[i], kTWarps);
+      mbar_init(&tfree[i], 1);
+      mbar_init(&drain[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kWarpShrink) tmem_alloc(s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;  // shrink accumulators at columns 0 and 128, expand at 256 and 384
+  const int n_tiles = p.plan.counts[0];
+  const int64_t n_units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
+  const int k_stages = p.bank.ka / KS;
+
+  if (warp < kXWarps) {
+    // ---------------- x: global -> registers -> split, swizzled shared memory ----------------
+    const int k = p.bank.k_in;
+    const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
+    const bool vec = p.x_vec != 0;
+    const int full_stages = vec ? k / KS : 0;  // stages that 16-byte loads can take whole
+    uint4 buf[XD][XV];
+    const XT* row[XV];
+    int passes = 0;  // of this unit: later ones have no rows
+    // the load cursor: unit u, its stage ks
+    int64_t u = blockIdx.x;
+    int ks = 0;
+    // The lines of a later stage into L2: DRAM's latency passes there instead of in registers.
+    auto prefetch = [&](int stage) {
+      const int c = stage * KS + col;
+      if ((col * (int)sizeof(XT)) % 128 == 0 && c < k) {
+#pragma unroll
+        for (int i = 0; i < XV; ++i)
+          if (i < passes) prefetch_l2(row[i] + c);
+      }
+    };
+    auto open = [&]() -> bool {  // the next unit with something to add from u on
+      for (; u < n_units; u += gridDim.x) {
+        const Unit un = get_unit(p, n_tiles, u);
+        if (un.rows <= 0 || un.ad.rank == 0) continue;
+        passes = (un.rows + XR - 1) / XR;
+#pragma unroll
+        for (int i = 0; i < XV; ++i)  // behind the last row: that row again
+          row[i] = static_cast<const XT*>(p.a.x) +
+                   (int64_t)p.plan.pos_row[un.pos0 + min(r0 + i * XR, un.rows - 1)] * p.a.ldx;
+        ks = 0;
+        for (int s = XD; s < XD + kXAhead; ++s) prefetch(s);
+        return true;
+      }
+      return false;
+    };
+    auto load = [&](uint4 (&v)[XV]) {
+      const int c = ks * KS + col;
+      if (ks < full_stages) {
+#pragma unroll
+        for (int i = 0; i < XV; ++i)
+          if (i < passes) v[i] = __ldg(reinterpret_cast<const uint4*>(row[i] + c));
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < XV; ++i) {
+        if (i >= passes) continue;
+        XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
+#pragma unroll
+        for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1)];
+#pragma unroll
+        for (int j = 0; j < XE; ++j) e[j] = c + j < k ? e[j] : as_type<XT>(0.0f);
+        if constexpr (PX == 2) {
+          v[i] = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
+          v[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                            h[6] | (uint32_t)h[7] << 16);
+        }
+      }
+    };
+    auto advance = [&]() -> bool {
+      if (++ks < k_stages) {
+        prefetch(ks + XD + kXAhead - 1);
+        return true;
+      }
+      u += gridDim.x;
+      return open();
+    };
+    Ring xr;
+    // this thread's 16-byte pieces of its first row in a slot (the rows of its passes are multiples of 8 apart)
+    const uint32_t at0 = (col / KC) * x_atom + r0 * 128 + (((col % KC) / 4) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
+    const bool second = col >= KC;  // 16-bit rows: these lanes store their second piece first (other banks)
+    static_assert(XR % 8 == 0, "swizzle");
+    auto store = [&](const uint4 (&v)[XV]) -> bool {
+      if (!warp_wait(&xempty[xr.slot], xr.parity ^ 1, abort_flag, err, 1u)) return false;
+      uint8_t* dst = sX + xr.slot * x_slot;
+#pragma unroll
+      for (int i = 0; i < XV; ++i) {
+        if (r0 + i * XR >= p.rt) break;
+        const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        if constexpr (PX == 2) {
+          float hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(e[j]), hi[j], lo[j]);
+          *reinterpret_cast<float4*>(dst + at0 + i * XR * 128) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<float4*>(dst + 2 * x_atom + at0 + i * XR * 128) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (std::is_same<XT, __half>::value) {
+              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
+              f[2 * j] = g.x, f[2 * j + 1] = g.y;
+            } else {
+              f[2 * j] = __uint_as_float(e[j] << 16), f[2 * j + 1] = __uint_as_float(e[j] & 0xffff0000u);
+            }
+          }
+          const float4 p0 = make_float4(f[0], f[1], f[2], f[3]), p1 = make_float4(f[4], f[5], f[6], f[7]);
+          *reinterpret_cast<float4*>(dst + (second ? at1 : at0) + i * XR * 128) = second ? p1 : p0;
+          *reinterpret_cast<float4*>(dst + (second ? at0 : at1) + i * XR * 128) = second ? p0 : p1;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&xfull[xr.slot]);
+      xr.next(p.x_slots);
+      return true;
+    };
+    bool more = open();
+    int ahead = 0;  // stages loaded and not stored
+#pragma unroll
+    for (int d = 0; d < XD; ++d) {
+#pragma unroll
+      for (int i = 0; i < XV; ++i) buf[d][i] = make_uint4(0, 0, 0, 0);
+      if (more) {
+        load(buf[d]);
+        ++ahead;
+        more = advance();
+      }
+    }
+    bool ok = true;
+    while (ok && ahead > 0) {
+#pragma unroll
+      for (int d = 0; d < XD; ++d) {
+        if (!ok || ahead == 0) break;
+        ok = store(buf[d]);
+        --ahead;
+        if (ok && more) {
+          load(buf[d]);
+          ++ahead;
+          more = advance();
+        }
+      }
+    }
+  } else if (warp < kWarpT) {
+    // ---------------- epilogue: base + accumulators -> y ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    const YT* base = static_cast<const YT*>(p.a.base);
+    YT* y = static_cast<YT*>(p.a.y);
+    const int quarter = warp & 3, half = (warp - kWarpEpi) >> 2, n_out = p.bank.n_out;
+    int32_t* rows = s_row + (warp - kWarpEpi) * 32;
+    uint32_t d = 0;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+      const Unit un = get_unit(p, n_tiles, u);
+      if (un.rows <= 0) continue;
+      if (un.ad.rank == 0 && p.a.base == p.a.y && p.a.ldb == p.a.ldy) continue;  // in place, nothing to add
+      if (un.ad.rank == 0) {
+        const int cols = min(n_out, un.c1 * 256) - un.c0 * 256;
+        for (int r = warp - kWarpEpi; r < un.rows; r += kEpiWarps) {
+          const int64_t row = p.plan.pos_row[un.pos0 + r];
+          for (int c = lane; c < cols; c += 32)
+            y[row * p.a.ldy + un.c0 * 256 + c] =
+                base ? base[row * p.a.ldb + un.c0 * 256 + c] : as_type<YT>(0.0f);
+        }
+        continue;
+      }
+      // this warp's rows: a half of the unit's (rt = 16: the first half takes all)
+      const int i0 = p.rt >= 32 ? half * (p.rt / 2) : half * 16, i1 = min(un.rows, i0 + (p.rt >= 32 ? p.rt / 2 : 16));
+      __syncwarp();
+      if (i0 < i1) rows[lane] = p.plan.pos_row[un.pos0 + min(i0 + lane, i1 - 1)];
+      __syncwarp();
+      for (int c = un.c0; ok && c < un.c1; ++c, ++d) {
+        const int ch = c * 256 + quarter * 64 + lane * 2;
+        if (base && c + 1 < un.c1 && i0 + lane < i1) {  // the next chunk's lines of a row into L2
+          const YT* nb = base + (int64_t)rows[lane] * p.a.ldb;
+          prefetch_l2(nb + min(ch - lane * 2 + 256, n_out - 1));
+          if (sizeof(YT) == 4) prefetch_l2(nb + min(ch - lane * 2 + 288, n_out - 1));
+        }
+        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (d & 1) * 128u;
+        auto wait = [&]() -> bool {
+          ok = warp_wait(&dfull[d & 1], (d >> 1) & 1, abort_flag, err, 2u);
+          if (ok) tc_fence_after();
+          return ok;
+        };
+        if (p.y_vec)
+          epilogue_rows<YT, 2>(base, y, rows, p.a.ldb, p.a.ldy, ch, n_out, i0, i1, acc, p.rt, wait);
+        else
+          epilogue_rows<YT, 1>(base, y, rows, p.a.ldb, p.a.ldy, ch, n_out, i0, i1, acc, p.rt, wait);
+        if (!ok) break;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dempty[d & 1]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp < kWarpShrink) {
+    // ---------------- t: TMEM -> scaled, split -> shared memory ----------------
+    const int quarter = warp & 3, row = quarter * 32 + lane;  // this lane's row of the unit
+    uint32_t q = 0;
+    Ring tr;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+      const Unit un = get_unit(p, n_tiles, u);
+      if (un.rows <= 0 || un.ad.rank == 0) continue;
+      float sc = un.ad.scale;
+      if (p.a.absmax && row < un.rows)
+        sc = __fmul_rn(sc, __fdiv_rn(__uint_as_float(p.a.absmax[p.a.per_seq ? p.plan.pos_seq[un.pos0 + row] : 0]),
+                                     127.0f));
+      const ShrinkAcc sa(p.bank.max_rank, un.ad.rank, PX == 2 || PW == 2, k_stages);
+      ok = warp_wait(&tafull[(q & (sa.bufs - 1))], (q >> (sa.bufs - 1)) & 1, abort_flag, err, 4u) &&
+           warp_wait(&tfree[tr.slot], tr.parity ^ 1, abort_flag, err, 8u);
+      if (!ok) break;
+      tc_fence_after();
+      if (quarter * 32 < un.rows) {
+        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + ((q & (sa.bufs - 1))) * 128u;
+        for (int j = 0; j < un.ad.rp; j += 8) {  // eight ranks: two 16-byte pieces of each plane
+          float t[8];
+          {
+            uint32_t v[8];
+            tmem_ld8(acc + (uint32_t)j, v);
+            tmem_wait_ld();
+            reg_barrier8(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = __uint_as_float(v[e]);
+          }
+          for (int k = 1; k < sa.parts; ++k) {
+            uint32_t v[8];
+            tmem_ld8(acc + (uint32_t)(k * sa.width + j), v);
+            tmem_wait_ld();
+            reg_barrier8(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = __fadd_rn(t[e], __uint_as_float(v[e]));
+          }
+          float hi[8], lo[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)  // ranks behind the last one meet zero columns of B: they have to be finite
+            split_tf32(j + e < un.ad.rank ? __fmul_rn(t[e], sc) : 0.0f, hi[e], lo[e]);
+          uint8_t* dst = sT + tr.slot * t_buf + (j / KC) * 2 * t_plane + row * 128;
+          if (row >= p.rt) continue;  // lanes without a row of t (units of 16 rows)
+          const int c0 = (j % KC) / 4, x = row & 7;
+          *reinterpret_cast<float4*>(dst + ((c0 ^ x) * 16)) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<float4*>(dst + (((c0 + 1) ^ x) * 16)) = make_float4(hi[4], hi[5], hi[6], hi[7]);
+          *reinterpret_cast<float4*>(dst + t_plane + ((c0 ^ x) * 16)) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<float4*>(dst + t_plane + (((c0 + 1) ^ x) * 16)) = make_float4(lo[4], lo[5], lo[6], lo[7]);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&taempty[(q & (sa.bufs - 1))]);
+        mbar_arrive(&tfull[tr.slot]);
+      }
+      tr.next(p.t_bufs);
+      ++q;
+    }
+  } else if (warp == kWarpShrink) {
+    // ---------------- tensor cores: t^T accumulators from x and A ----------------
+    if (elect_lane()) {
+      Ring xr, ar;
+      uint32_t q = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+        const Unit un = get_unit(p, n_tiles, u);
+        if (un.rows <= 0 || un.ad.rank == 0) continue;
+        const ShrinkAcc sa(p.bank.max_rank, un.ad.rank, PX == 2 || PW == 2, k_stages);
+        const uint32_t set = q & (sa.bufs - 1), id = idesc_tf32(128, sa.width);
+        ok = stage_wait(&taempty[set], ((q >> (sa.bufs - 1)) & 1) ^ 1, abort_flag, err, 16u);
+        tc_fence_after();
+        const uint32_t acc0 = tmem + set * 128u, acc_lo = acc0 + (uint32_t)(sa.hi_parts * sa.width);
+        int c = 0;
+        for (int part = 0; ok && part < sa.hi_parts; ++part) {
+          const uint32_t acc = acc0 + (uint32_t)(part * sa.width);
+          const int end = k_stages * (part + 1) / sa.hi_parts;
+          for (uint32_t more = 0; c < end; ++c) {
+            ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u) &&
+                 stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot), w0 = desc_lo(smem_u32(sA) + ar.slot * a_slot);
+            const uint32_t lo_x = x_atom >> 3, lo_w = a_rows << 4;  // from the hi to the lo plane
+#pragma unroll
+            for (int s = 0; s < KS / 8; ++s) {
+              const uint32_t x = x0 + s / 4 * (x_atom >> 4) + s % 4 * 2, w = w0 + s / 4 * (a_rows << 3) + s % 4 * 2;
+              umma_tf32(acc, desc_at(x), desc_at(w), id, s > 0 ? 1 : more);
+              if (PX == 2) umma_tf32(acc_lo, desc_at(x + lo_x), desc_at(w), id, c > 0 || s > 0);
+              if (PW == 2) umma_tf32(acc_lo, desc_at(x), desc_at(w + lo_w), id, PX == 2 || c > 0 || s > 0);
+            }
+            more = 1;
+            umma_commit(&xempty[xr.slot]);
+            umma_commit(&aempty[ar.slot]);
+            xr.next(p.x_slots);
+            ar.next(p.a_slots);
+          }
+        }
+        if (ok) umma_commit(&tafull[set]);
+        ++q;
+      }
+      // every MMA and every commit's arrival is done before the CTA's memory goes
+      umma_commit(&drain[0]);
+      mbar_wait_drain(&drain[0], 0);
+    }
+  } else if (warp == kWarpExpand) {
+    // ---------------- tensor cores: result accumulators from B and t ----------------
+    if (elect_lane()) {
+      const uint32_t id = idesc_tf32(128, p.rt);
+      Ring br, tr;
+      uint32_t d = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+        const Unit un = get_unit(p, n_tiles, u);
+        if (un.rows <= 0 || un.ad.rank == 0) continue;
+        ok = stage_wait(&tfull[tr.slot], tr.parity, abort_flag, err, 128u);
+        tc_fence_after();
+        for (int c = un.c0; ok && c < un.c1; ++c, ++d) {
+          ok = stage_wait(&dempty[d & 1], ((d >> 1) & 1) ^ 1, abort_flag, err, 256u);
+          tc_fence_after();
+          for (int g = 0; ok && g < 2; ++g) {  // even, then odd channels
+            const uint32_t acc = tmem + 256u + (d & 1) * 128u + (uint32_t)(g * p.rt);
+            uint32_t t = desc_lo(smem_u32(sT) + tr.slot * t_buf), more = 0;
+            for (int left = un.ad.rp / 8; ok && left > 0; left -= KC / 8) {
+              ok = stage_wait(&bfull[br.slot], br.parity, abort_flag, err, 1024u);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t w = desc_lo(smem_u32(sB) + br.slot * b_slot);
+#pragma unroll
+              for (int s = 0; s < KC / 8; ++s) {
+                if (s >= left) break;
+                umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + (t_plane >> 4) + 2 * s), id, s > 0 ? 1 : more);
+                if (PW == 2) umma_tf32(acc, desc_at(w + (kBPlane >> 4) + 2 * s), desc_at(t + 2 * s), id, 1);
+                umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + 2 * s), id, 1);
+              }
+              more = 1;
+              umma_commit(&bempty[br.slot]);
+              br.next(p.b_slots);
+              t += 2 * t_plane >> 4;
+            }
+          }
+          if (ok) umma_commit(&dfull[d & 1]);
+        }
+        if (ok) umma_commit(&tfree[tr.slot]);
+        tr.next(p.t_bufs);
+      }
+      umma_commit(&drain[1]);
+      mbar_wait_drain(&drain[1], 0);
+    }
+  } else if (warp <= kWarpB && lane == 0) {
+    // ---------------- weights: bulk copies of the bank's tiles (A's, or B's) ----------------
+    const bool is_a = warp == kWarpA;
+    uint8_t* ring = is_a ? sA : sB;
+    const uint32_t slots = is_a ? p.a_slots : p.b_slots, slot = is_a ? a_slot : b_slot;
+    const uint32_t pieces = is_a ? 2 * PW : PW, to_piece = is_a ? a_rows * 128 : kBPlane;  // per slot
+    uint64_t *full = is_a ? afull : bfull, *empty = is_a ? aempty : bempty;
+    Ring r;
+    uint32_t issued = 0;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+      const Unit un = get_unit(p, n_tiles, u);
+      if (un.rows <= 0 || un.ad.rank == 0) continue;
+      const int rcs = (un.ad.rp + KC - 1) / KC;
+      const uint32_t bytes = is_a ? un.ad.rank * 128 : kBPlane;  // of a piece
+      const uint8_t* src = is_a ? un.ad.ta : un.ad.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
+      for (int n = is_a ? k_stages : (un.c1 - un.c0) * 2 * rcs; n > 0; --n) {
+        ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&full[r.slot], bytes * pieces);
+        for (uint32_t i = 0; i < pieces; ++i, src += bytes)
+          bulk_load(ring + r.slot * slot + i * to_piece, src, bytes, &full[r.slot]);
+        r.next(slots);
+        ++issued;
+      }
+    }
+    // copies in flight land before the CTA's shared memory is released
+    for (uint32_t i = issued > slots ? issued - slots : 0; i < issued; ++i)
+      mbar_wait_drain(&full[i % slots], (i / slots) & 1);
+  }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpShrink) tmem_dealloc(tmem, 512);
+}
+
+// The bank's weights as the kernel's tiles, tf32 planes (hi, and lo for float32
+// weights) of rows of 32 values whose 16-byte pieces are swizzled by the row
+// number; zeros outside. A: [k stage][plane][2 x 32 channels][rank rows]. B:
+// [chunk of 256 channels][even, odd][32 ranks][plane][128 rows], row i of a
+// chunk's tile g being channel 2 i + g.
+template <class WT>
+__global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int ka, int planes) {
+  const int64_t na = (int64_t)ad.rank * ka;
+  const int rcs = (ad.rp + KC - 1) / KC, tiles = (n_out + 255) / 256 * 2 * rcs;
+  const int64_t nb = (int64_t)tiles * 128 * KC;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < na + nb; i += (int64_t)gridDim.x * blockDim.x) {
+    float v = 0.0f;
+    int row, c;
+    uint8_t* tile;
+    int64_t plane;  // bytes from the hi to the lo plane
+    if (i < na) {
+      row = (int)(i / ka);
+      const int kk = (int)(i % ka);
+      c = kk % KC;
+      const int64_t atom = (int64_t)ad.rank * 128;
+      plane = 2 * atom;
+      tile = const_cast<uint8_t*>(ad.ta) + (int64_t)(kk / KS) * planes * plane + kk % KS / KC * atom;
+      if (kk < k_in) v = as_f32(static_cast<const WT*>(ad.a)[i]);
+    } else {
+      const int64_t b = i - na, t = b / (128 * KC);
+      row = (int)(b % (128 * KC)) / KC;
+      c = (int)(b % KC);
+      plane = kBPlane;
+      tile = const_cast<uint8_t*>(ad.tb) + t * planes * plane;
+      const int64_t n = t / (2 * rcs) * 256 + 2 * row + t / rcs % 2;
+      const int j = (int)(t % rcs) * KC + c;
+      if (n < n_out && j < ad.rank) v = as_f32(static_cast<const WT*>(ad.b)[n * ad.rp + j]);
+    }
+    float* dst = reinterpret_cast<float*>(tile + (int64_t)row * 128 + (((c >> 2) ^ (row & 7)) * 16) + (c & 3) * 4);
+    if (planes == 2) {
+      float hi, lo;
+      split_tf32(v, hi, lo);
+      dst[0] = hi;
+      dst[plane / 4] = lo;
+    } else {
+      dst[0] = v;
+    }
+  }
+}
+
+template <class XT, class YT>
+cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
+  constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;
+  const int planes = p.bank.wtype == kDtF32 ? 2 : 1;
+  const int chunks = (p.bank.n_out + 255) / 256;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  p.rt = kRt;
+  p.splits = 1;
+  while (p.rt > 16 && (int64_t)n_tiles * (kAdapterTileRows / p.rt) < sms) p.rt /= 2;
+  while (p.splits < chunks && (int64_t)n_tiles * (kAdapterTileRows / p.rt) * (p.splits + 1) <= sms) ++p.splits;
+  // Shared memory: rings of two to four slots, and a second buffer of t when there is room.
+  const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = planes * 2 * ((p.bank.max_rank + 15) / 16 * 16) * 128;
+  int smem = 0;
+  for (;; p.rt /= 2) {
+    const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * 2 * p.rt * 128;
+    int left = kMaxSmem - 1024 - kMiscBytes - 2 * (planes * kBPlane + a_slot + x_slot) - t_buf;
+    if (left < 0) continue;
+    p.t_bufs = 1, p.a_slots = p.b_slots = p.x_slots = 2;
+    for (int round = 0; round < 2; ++round) {
+      if (left >= x_slot) left -= x_slot, ++p.x_slots;
+      if (round == 0 && left >= t_buf) left -= t_buf, ++p.t_bufs;
+      if (left >= a_slot) left -= a_slot, ++p.a_slots;
+      if (left >= planes * kBPlane) left -= planes * kBPlane, ++p.b_slots;
+    }
+    smem = kMaxSmem - left;
+    break;
+  }
+  p.x_vec = (reinterpret_cast<uintptr_t>(p.a.x) & 15) == 0 && (p.a.ldx * sizeof(XT)) % 16 == 0;
+  p.y_vec = p.bank.n_out % 2 == 0 && p.a.ldy % 2 == 0 && (!p.a.base || p.a.ldb % 2 == 0) &&
+            ((reinterpret_cast<uintptr_t>(p.a.y) | reinterpret_cast<uintptr_t>(p.a.base)) & (2 * sizeof(YT) - 1)) == 0;
+  e = cudaFuncSetAttribute(lowrank_tc_kernel<XT, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
+  lowrank_tc_kernel<XT, YT><<<(unsigned)(units < sms ? units : sms), kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t lowrank_tile_bytes_a(int rank, int ka, int wtype) {
+  return (size_t)(ka / KC) * rank * 128 * (wtype == kDtF32 ? 2 : 1);
+}
+size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype) {
+  return (size_t)((n_out + 255) / 256 * 2) * ((rp + KC - 1) / KC) * kBPlane * (wtype == kDtF32 ? 2 : 1);
+}
+
+cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, int ka, int wtype, cudaStream_t st) {
+  if (ad.rank <= 0) return cudaSuccess;
+  const int planes = wtype == kDtF32 ? 2 : 1;
+  const int64_t n = (int64_t)ad.rank * ka + (int64_t)((n_out + 255) / 256 * 2) * ((ad.rp + KC - 1) / KC) * 128 * KC;
+  const unsigned grid = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
+  if (wtype == kDtF32) lowrank_tiles_kernel<float><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+  else if (wtype == kDtF16) lowrank_tiles_kernel<__half><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+  else lowrank_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles, const LowRankArgs& a,
+                              uint32_t* err, cudaStream_t st) {
+  if (n_tiles <= 0) return cudaSuccess;
+  TcParams p{};
+  p.bank = bank;
+  p.plan = plan;
+  p.a = a;
+  p.err = err;
+  if (a.xtype == kDtF32 && a.ytype == kDtF32) return tc_types<float, float>(p, n_tiles, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF16) return tc_types<__half, __half>(p, n_tiles, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF32) return tc_types<__half, float>(p, n_tiles, st);
+  if (a.xtype == kDtBF16 && a.ytype == kDtBF16) return tc_types<__nv_bfloat16, __nv_bfloat16>(p, n_tiles, st);
+  if (a.xtype == kDtBF16 && a.ytype == kDtF32) return tc_types<__nv_bfloat16, float>(p, n_tiles, st);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace sem
