@@ -15,9 +15,10 @@ constexpr int kAdapterTileRows = 64;
 constexpr int kAdapterSmallRows = 16;
 
 // Up to kAdapterTileRows positions [pos0, pos0 + rows) of the order by adapter
-// that all use `adapter` (-1: none).
-struct AdapterTile {
-  int32_t adapter, pos0, rows;
+// that all use `adapter` (-1: none). row0: their rows are [row0, row0 + rows),
+// or -1 when they do not follow each other.
+struct alignas(16) AdapterTile {
+  int32_t adapter, pos0, rows, row0;
 };
 
 // The rows of a batch ordered by adapter: its sequences sorted by adapter
@@ -66,6 +67,10 @@ inline AdapterPlanHost adapter_plan_build(const int32_t* offsets, const int32_t*
     at += offsets[p.order[i] + 1] - offsets[p.order[i]];
   }
   p.pos[n_seqs] = p.rows = at;
+  auto row_at = [&](int32_t q) {  // the last sequence that starts at or before position q holds it
+    const int32_t i = (int32_t)(std::upper_bound(p.pos.begin(), p.pos.end() - 1, q) - p.pos.begin()) - 1;
+    return offsets[p.order[i]] + (q - p.pos[i]);
+  };
   for (int32_t i = 0; i < n_seqs;) {  // one group of sequences per adapter
     const int32_t a = adapters[p.order[i]];
     int32_t j = i;
@@ -74,7 +79,9 @@ inline AdapterPlanHost adapter_plan_build(const int32_t* offsets, const int32_t*
     if (end > p.pos[i]) p.max_adapter = std::max(p.max_adapter, a);
     for (int32_t r = p.pos[i]; r < end;) {
       const int32_t n = std::min(kAdapterTileRows, end - r);
-      (n <= kAdapterSmallRows ? p.small : p.large).push_back(AdapterTile{a, r, n});
+      // the rows of a group increase with its positions
+      const int32_t first = row_at(r), last = row_at(r + n - 1);
+      (n <= kAdapterSmallRows ? p.small : p.large).push_back(AdapterTile{a, r, n, last - first == n - 1 ? first : -1});
       r += n;
     }
     i = j;

@@ -41,7 +41,7 @@ int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapte
   p->max_seqs = max_seqs;
   const int64_t large = adapter_plan_max_large(max_rows, max_seqs);
   // one upload: counts, sequences (pos, row0, seq, adapter), tiles
-  p->up_bytes = 16 + ((size_t)4 * max_seqs + 4) * 4 + ((size_t)large + max_seqs) * sizeof(AdapterTile);
+  p->up_bytes = 16 + (size_t)round_up((size_t)4 * max_seqs + 4, 4) * 4 + ((size_t)large + max_seqs) * sizeof(AdapterTile);
   cudaError_t e = p->up.ensure(p->up_bytes);
   if (e == cudaSuccess) e = p->maps.ensure((size_t)3 * (max_rows > 0 ? max_rows : 1) * 4);
   if (e == cudaSuccess) e = p->staging.ensure(p->up_bytes);
@@ -57,7 +57,7 @@ int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapte
 
 AdapterPlanDev plan_device(const sem_adapter_plan* p) {
   const uint8_t* up = p->up.as<uint8_t>();
-  const AdapterTile* tiles = reinterpret_cast<const AdapterTile*>(up + 16 + ((size_t)4 * p->max_seqs + 4) * 4);
+  const AdapterTile* tiles = reinterpret_cast<const AdapterTile*>(up + 16 + (size_t)round_up((size_t)4 * p->max_seqs + 4, 4) * 4);
   const int32_t* maps = p->maps.as<int32_t>();
   return AdapterPlanDev{reinterpret_cast<const int32_t*>(up), tiles,
                         tiles + adapter_plan_max_large(p->max_rows, p->max_seqs), maps, maps + p->max_rows,
@@ -78,7 +78,7 @@ int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapter
   AdapterPlanHost h = adapter_plan_build(offsets, adapters, n_seqs);
   // the previous upload has left the staging buffer
   SEM_CUDA(cudaEventSynchronize(p->staged));
-  const size_t seq_ints = (size_t)4 * p->max_seqs + 4;
+  const size_t seq_ints = (size_t)round_up((size_t)4 * p->max_seqs + 4, 4);  // the tiles start on 16 bytes
   uint8_t* s = p->staging.as<uint8_t>();
   int32_t* counts = reinterpret_cast<int32_t*>(s);
   counts[0] = (int32_t)h.large.size();

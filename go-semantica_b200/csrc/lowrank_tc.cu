@@ -11,7 +11,7 @@
 //
 // Numbers. The operands are tf32 (11 significant bits): fp16, bf16 and INT8
 // codes are exact in it; a float32 value v goes in as two parts, hi = v cut to
-// 11 bits and lo = v - hi (exact, of which the tensor core keeps 11 bits), and
+// 11 bits and lo = v - hi cut to 11 bits, and
 // hi hi + hi lo + lo hi are accumulated in float32 in TMEM, so products keep at
 // least 21 bits. t stays float32 between the products (hi and lo again). Only
 // y's own rounding loses bits.
@@ -20,15 +20,18 @@
 // needs 2 r (k + n) flops (r = 16, 768 x 768, float32: 9.2 KB against 49
 // kflop, two products each: 0.02 of the tensor pipe). So the work is to keep
 // loads in flight and every other role short:
-//   - X warps (8): rows of x through registers (32 KB in flight, any row order
-//     and alignment), split and stored 128-byte swizzled;
+//   - X warps (8): rows of x (any order and alignment) by asynchronous copies
+//     to where their operand goes, 128-byte swizzled, then split in place;
 //   - two copy threads: the adapter's A and B tiles, which the bank keeps as
 //     tf32 planes in the swizzled layout, with one bulk copy per plane;
 //   - a shrink and an expand MMA thread, so that the shrink of later units
 //     goes on while the epilogue holds up the expand of an earlier one;
 //   - T warps (2): t from TMEM, scaled, split, to shared memory;
-//   - epilogue warps (8): base prefetched ahead of the accumulators.
-// One persistent CTA per SM.
+//   - epilogue warps (16): base by asynchronous copies into a ring per warp,
+//     ahead of the accumulators and across units.
+// One persistent CTA per SM. Loads into registers in place of the asynchronous
+// copies were measured: what is in flight then has to fit the 20-odd KB of L1
+// that the shared memory leaves, 148 us against MEAS_NEW (128 x 512 rows).
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -41,22 +44,20 @@ namespace sem {
 
 namespace {
 
-constexpr int kXWarps = 8, kEpiWarps = 8, kTWarps = 2;
+constexpr int kXWarps = 8, kEpiWarps = 16, kTWarps = 2;
 constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
 constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1;
 constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA and copy warps, two idle
-// Registers: 768 threads get 80 each at launch; the last two warpgroups give
-// 32 back (256 x 48), the epilogue's take them (256 x 112).
-static_assert(kWarpB < kThreads / 32 && 256 * 80 + 256 * 112 + 256 * 48 <= kThreads * 80, "register split");
+static_assert(kThreads == 1024, "64 registers each");
 static_assert(kWarpEpi % 4 == 0 && kWarpT % 4 == 0, "TMEM lane quarters go by warp index");
 constexpr int KC = 32;   // tf32 per swizzled 128-byte row
 constexpr int KS = 64;   // input channels per stage: two such rows
 constexpr int kRt = 64;  // rows per unit at most
 static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile or a part of one");
-constexpr int kMaxSlots = 4;
-constexpr int kXAhead = 2;  // stages of x prefetched to L2 ahead of the loads
+constexpr int kMaxSlots = 8;
 constexpr int kBPlane = 128 * 128;  // one plane of a slot of B: 128 channels x 128 bytes
-constexpr int kMiscBytes = 512 + kEpiWarps * 32 * 4;
+constexpr int kMiscBytes = 512;
+constexpr int kEpiRows = 8;  // rows per batch of an epilogue warp's ring of base
 constexpr int kMaxSmem = 232448;  // an MMA reads 128 rows from a slot's start: a short slot's run on into sW and sT
 
 __device__ uint32_t g_lowrank_error;
@@ -140,14 +141,33 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, stage_wait(bar, parity, abort_flag, err, code));
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// Asynchronous copies global -> shared: 16 bytes of which the first `bytes`
+// come from memory (the rest are zeros), or 4 bytes.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// All but the last n of this thread's copy groups are complete (n < 6).
+__device__ __forceinline__ void copy_wait(int n) {
+  switch (n) {
+    case 0: cp_async_wait<0>(); break;
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    case 4: cp_async_wait<4>(); break;
+    default: cp_async_wait<5>(); break;
+  }
+}
 
 // v = hi + lo: hi the upper 11 significant bits. |lo| < 2^-11 * 2^128 < 2e35,
 // so the maximum only replaces the NaN that an infinite v leaves in lo (which
-// would turn an infinite result into NaN); a NaN v stays one in hi.
+// would turn an infinite result into NaN); a NaN v stays one in hi. lo's bits
+// behind its own 11 are cut too: an operand is a tf32 value.
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
-  lo = fmaxf(__fsub_rn(v, hi), -2e35f);
+  lo = __uint_as_float(__float_as_uint(fmaxf(__fsub_rn(v, hi), -2e35f)) & 0xffffe000u);
 }
 
 template <class T>
@@ -176,11 +196,6 @@ __device__ __forceinline__ void reg_barrier8(uint32_t (&r)[8]) {
                : "memory");
 }
 
-__device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-__device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
-__device__ __forceinline__ void reg_barriern(uint32_t (&r)[16]) { reg_barrier16(r); }
-__device__ __forceinline__ void reg_barriern(uint32_t (&r)[8]) { reg_barrier8(r); }
-
 // The 256 TMEM columns of t's accumulators. The tensor core cuts every sum it
 // forms, an error that grows with the number of sums into one accumulator and
 // with its size; so the products run into up to four accumulators (the low
@@ -200,6 +215,7 @@ struct ShrinkAcc {
 struct Unit {
   LowRankAdapter ad;
   int32_t pos0, rows;  // positions; rows <= 0: nothing
+  int32_t row0;        // their rows follow each other from here, or -1
   int32_t c0, c1;      // chunks of 256 output channels
 };
 
@@ -209,8 +225,10 @@ struct TcParams {
   LowRankArgs a;
   int32_t rt, splits;        // rows per unit (16, 32 or 64), shares of the output channels
   int32_t x_slots, a_slots, b_slots, t_bufs;  // ring depths
-  int32_t x_vec;  // rows of x start on 16 bytes
-  int32_t y_vec;  // channels of base and y can be accessed in pairs
+  int32_t epi_ring;  // bytes of an epilogue warp's ring: 2048 or 4096
+  int32_t x_vec;   // rows of x start on 16 bytes
+  int32_t b_copy;  // bytes of a copy that base's rows are aligned for: 16, 4 or 2 (none, element loads)
+  int32_t y_pair;  // y's channels can be stored in pairs
   uint32_t* err;
 };
 
@@ -224,6 +242,7 @@ __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t
   const int off = (int)(v / n_tiles) * p.rt;
   r.pos0 = tl.pos0 + off;
   r.rows = min(p.rt, tl.rows - off);
+  r.row0 = tl.row0 < 0 ? -1 : tl.row0 + off;
   const int chunks = (p.bank.n_out + 255) / 256;
   r.c0 = chunks * split / p.splits;
   r.c1 = chunks * (split + 1) / p.splits;
@@ -233,83 +252,26 @@ __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t
   return r;
 }
 
-// One chunk of a warp: rows [i0, i1) of the unit, channels ch and ch + 1 of
-// each lane, whose accumulators are the columns at `acc` (even channels) and
-// rt further (odd). `wait` (the accumulators are complete) is called between
-// the first loads of base and their use. VEC 2: the pair is accessed as one.
-template <class YT, int VEC, class Wait>
-__device__ __forceinline__ void epilogue_rows(const YT* base, YT* y, const int32_t* rows, int64_t ldb, int64_t ldy,
-                                              int ch, int n_out, int i0, int i1, uint32_t acc, int rt, Wait wait) {
-  struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
-  constexpr int B = VEC == 2 ? 16 : 8;
-  // Loads without conditions (rows behind the last one repeat it, channels behind n_out read the last ones), held in
-  // their own type: a condition or a conversion in between would make each load wait for the one before.
-  const int c0 = VEC == 2 ? min(ch, n_out - 2) : min(ch, n_out - 1), c1 = min(ch + 1, n_out - 1);
-  Pair nxt[B];
-  auto fetch = [&](int i) {
-    if (base) {
-#pragma unroll
-      for (int j = 0; j < B; ++j) {
-        const YT* b = base + (int64_t)rows[i - i0 + j] * ldb;
-        if (VEC == 2) nxt[j] = *reinterpret_cast<const Pair*>(b + c0);
-        else nxt[j].e[0] = b[c0], nxt[j].e[1] = b[c1];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < B; ++j) nxt[j].e[0] = nxt[j].e[1] = as_type<YT>(0.0f);
-    }
-  };
-  if (i0 < i1) fetch(i0);
-  if (!wait()) return;
-  for (int i = i0; i < i1; i += B) {
-    uint32_t v0[B], v1[B];
-    tmem_ldn(acc + (uint32_t)i, v0);
-    tmem_ldn(acc + (uint32_t)(rt + i), v1);
-    tmem_wait_ld();
-    reg_barriern(v0);
-    reg_barriern(v1);
-    Pair out[B];
-#pragma unroll
-    for (int j = 0; j < B; ++j) {
-      out[j].e[0] = as_type<YT>(__fadd_rn(as_f32(nxt[j].e[0]), __uint_as_float(v0[j])));
-      out[j].e[1] = as_type<YT>(__fadd_rn(as_f32(nxt[j].e[1]), __uint_as_float(v1[j])));
-    }
-    if (i + B < i1) fetch(i + B);
-    const int live = i1 - i;
-#pragma unroll
-    for (int j = 0; j < B; ++j) {
-      if (j >= live) break;
-      YT* d = y + (int64_t)rows[i - i0 + j] * ldy + ch;
-      if (VEC == 2) {
-        if (ch < n_out) *reinterpret_cast<Pair*>(d) = out[j];
-      } else {
-        if (ch < n_out) d[0] = out[j].e[0];
-        if (ch + 1 < n_out) d[1] = out[j].e[1];
-      }
-    }
-  }
-}
-
 template <class XT, class YT>
 __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_constant__ TcParams p) {
   constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;  // planes of x
-  constexpr int XE = 16 / sizeof(XT);                         // elements of one 16-byte load
-  constexpr int XL = KS / XE;                                 // loads per row and stage
+  constexpr int XE = 16 / sizeof(XT);                         // elements of a 16-byte copy
+  constexpr int XL = KS / XE;                                 // copies per row and stage
   constexpr int XR = kXWarps * 32 / XL;                       // rows per pass of the X warps
   constexpr int XV = kRt / XR;                                // passes
-  constexpr int XD = 8 / XV;                                  // stages in flight: 8 loads per thread, 32 KB per SM
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int PW = p.bank.wtype == kDtF32 ? 2 : 1;  // planes of the weights
   const int x_atom = p.rt * 128, x_slot = PX * 2 * x_atom;  // [plane][32 channels][rt rows][128 B]
-  const int a_rows = (p.bank.max_rank + 15) & ~15, a_slot = PW * 2 * a_rows * 128, b_slot = PW * kBPlane;
+  const int a_slot = ((p.bank.max_rank + 15) & ~15) * 128;  // a piece of A: the ranks of 32 channels of a plane
   const int t_plane = p.rt * 128, t_chunks = (p.bank.max_rank + KC - 1) / KC;  // [chunk][hi, lo][rt rows][128 B]
   uint8_t* sX = smem;
   uint8_t* sA = sX + p.x_slots * x_slot;
   uint8_t* sB = sA + p.a_slots * a_slot;
-  uint8_t* sT = sB + p.b_slots * b_slot;
+  uint8_t* sT = sB + p.b_slots * kBPlane;
   const int t_buf = t_chunks * 2 * t_plane;
-  uint8_t* misc = sT + p.t_bufs * t_buf;
+  uint8_t* sE = sT + p.t_bufs * t_buf;
+  uint8_t* misc = sE + kEpiWarps * p.epi_ring;
   uint64_t* xfull = reinterpret_cast<uint64_t*>(misc);
   uint64_t* xempty = xfull + kMaxSlots;
   uint64_t* afull = xempty + kMaxSlots;   // weights of the shrink and of the expand
@@ -325,7 +287,6 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   uint64_t* drain = dempty + 2;           // [2] the MMA threads' last MMAs
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
-  int32_t* s_row = reinterpret_cast<int32_t*>(misc + 512);      // [epilogue warp][64] rows of its half of the unit
   uint32_t* err = p.err ? p.err : &g_lowrank_error;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -360,86 +321,88 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   const int k_stages = p.bank.ka / KS;
 
   if (warp < kXWarps) {
-    // ---------------- x: global -> registers -> split, swizzled shared memory ----------------
+    // ---------------- x: global -> swizzled shared memory, split in place ----------------
     const int k = p.bank.k_in;
     const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
-    const bool vec = p.x_vec != 0;
-    const int full_stages = vec ? k / KS : 0;  // stages that 16-byte loads can take whole
-    uint4 buf[XD][XV];
+    const int full_stages = p.x_vec ? k / KS : 0;  // stages that 16-byte copies can take
     const XT* row[XV];
-    int passes = 0;  // of this unit: later ones have no rows
-    // the load cursor: unit u, its stage ks
+    // the cursor of the copies: unit u, its stage ks
     int64_t u = blockIdx.x;
-    int ks = 0;
-    // The lines of a later stage into L2: DRAM's latency passes there instead of in registers.
-    auto prefetch = [&](int stage) {
-      const int c = stage * KS + col;
-      if ((col * (int)sizeof(XT)) % 128 == 0 && c < k) {
-#pragma unroll
-        for (int i = 0; i < XV; ++i)
-          if (i < passes) prefetch_l2(row[i] + c);
-      }
-    };
+    int ks = 0, passes = 0;
     auto open = [&]() -> bool {  // the next unit with something to add from u on
       for (; u < n_units; u += gridDim.x) {
         const Unit un = get_unit(p, n_tiles, u);
         if (un.rows <= 0 || un.ad.rank == 0) continue;
-        passes = (un.rows + XR - 1) / XR;
+        passes = (un.rows + XR - 1) / XR;  // later ones have no rows
 #pragma unroll
         for (int i = 0; i < XV; ++i)  // behind the last row: that row again
+        {
+          const int r = min(r0 + i * XR, un.rows - 1);
           row[i] = static_cast<const XT*>(p.a.x) +
-                   (int64_t)p.plan.pos_row[un.pos0 + min(r0 + i * XR, un.rows - 1)] * p.a.ldx;
+                   (int64_t)(un.row0 >= 0 ? un.row0 + r : p.plan.pos_row[un.pos0 + r]) * p.a.ldx;
+        }
         ks = 0;
-        for (int s = XD; s < XD + kXAhead; ++s) prefetch(s);
         return true;
       }
       return false;
     };
-    auto load = [&](uint4 (&v)[XV]) {
-      const int c = ks * KS + col;
-      if (ks < full_stages) {
+    // This thread's 16-byte pieces of its first row in a slot (its other rows are multiples of 8 further). A copy
+    // of 16-bit values lands where the first or, in lanes of the upper 32 channels, the second of its two pieces
+    // goes, and that piece is written first: the lanes of a row then touch different banks.
+    static_assert(XR % 8 == 0, "swizzle");
+    const bool upper = PX == 1 && col >= KC;
+    const uint32_t at0 = (col / KC) * x_atom + r0 * 128 + (((col % KC) / 4) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
+    const uint32_t land = upper ? at1 : at0;
+    Ring ir, xr;  // copies issued, stages done
+    bool ok = true, more = open();
+    int pending = 0;
+    auto issue = [&]() {  // the cursor's stage, one group (an empty one at the end)
+      if (more) {
+        ok = warp_wait(&xempty[ir.slot], ir.parity ^ 1, abort_flag, err, 1u);
+        if (!ok) return;
+        uint8_t* dst = sX + ir.slot * x_slot + land;
+        const int c = ks * KS + col;
 #pragma unroll
-        for (int i = 0; i < XV; ++i)
-          if (i < passes) v[i] = __ldg(reinterpret_cast<const uint4*>(row[i] + c));
-        return;
-      }
+        for (int i = 0; i < XV; ++i) {
+          if (i >= passes || r0 + i * XR >= p.rt) break;
+          if (ks < full_stages) {
+            copy16(smem_u32(dst) + i * XR * 128, row[i] + c, 16);
+          } else {
+            XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
 #pragma unroll
-      for (int i = 0; i < XV; ++i) {
-        if (i >= passes) continue;
-        XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
+            for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1)];
+            uint32_t v[4];
+            if constexpr (PX == 2) {
 #pragma unroll
-        for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1)];
+              for (int j = 0; j < 4; ++j) v[j] = c + j < k ? __float_as_uint(e[j]) : 0u;
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
 #pragma unroll
-        for (int j = 0; j < XE; ++j) e[j] = c + j < k ? e[j] : as_type<XT>(0.0f);
-        if constexpr (PX == 2) {
-          v[i] = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
-        } else {
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
-          v[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                            h[6] | (uint32_t)h[7] << 16);
+              for (int j = 0; j < 4; ++j)
+                v[j] = (c + 2 * j < k ? h[2 * j] : 0u) | (c + 2 * j + 1 < k ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+            }
+            *reinterpret_cast<uint4*>(dst + i * XR * 128) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        ir.next(p.x_slots);
+        ++pending;
+        if (++ks == k_stages) {
+          u += gridDim.x;
+          more = open();
         }
       }
+      cp_async_commit();
     };
-    auto advance = [&]() -> bool {
-      if (++ks < k_stages) {
-        prefetch(ks + XD + kXAhead - 1);
-        return true;
-      }
-      u += gridDim.x;
-      return open();
-    };
-    Ring xr;
-    // this thread's 16-byte pieces of its first row in a slot (the rows of its passes are multiples of 8 apart)
-    const uint32_t at0 = (col / KC) * x_atom + r0 * 128 + (((col % KC) / 4) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
-    const bool second = col >= KC;  // 16-bit rows: these lanes store their second piece first (other banks)
-    static_assert(XR % 8 == 0, "swizzle");
-    auto store = [&](const uint4 (&v)[XV]) -> bool {
-      if (!warp_wait(&xempty[xr.slot], xr.parity ^ 1, abort_flag, err, 1u)) return false;
+    const int depth = p.x_slots - 1;
+    for (int d = 0; ok && d < depth; ++d) issue();
+    while (ok && pending > 0) {
+      copy_wait(depth - 1);  // the oldest stage of this thread has landed
       uint8_t* dst = sX + xr.slot * x_slot;
 #pragma unroll
       for (int i = 0; i < XV; ++i) {
         if (r0 + i * XR >= p.rt) break;
-        const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        const uint4 v = *reinterpret_cast<const uint4*>(dst + land + i * XR * 128);
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
         if constexpr (PX == 2) {
           float hi[4], lo[4];
 #pragma unroll
@@ -458,56 +421,113 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             }
           }
           const float4 p0 = make_float4(f[0], f[1], f[2], f[3]), p1 = make_float4(f[4], f[5], f[6], f[7]);
-          *reinterpret_cast<float4*>(dst + (second ? at1 : at0) + i * XR * 128) = second ? p1 : p0;
-          *reinterpret_cast<float4*>(dst + (second ? at0 : at1) + i * XR * 128) = second ? p0 : p1;
+          *reinterpret_cast<float4*>(dst + land + i * XR * 128) = upper ? p1 : p0;
+          *reinterpret_cast<float4*>(dst + (land ^ 16) + i * XR * 128) = upper ? p0 : p1;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&xfull[xr.slot]);
       xr.next(p.x_slots);
-      return true;
-    };
-    bool more = open();
-    int ahead = 0;  // stages loaded and not stored
-#pragma unroll
-    for (int d = 0; d < XD; ++d) {
-#pragma unroll
-      for (int i = 0; i < XV; ++i) buf[d][i] = make_uint4(0, 0, 0, 0);
-      if (more) {
-        load(buf[d]);
-        ++ahead;
-        more = advance();
-      }
+      --pending;
+      issue();
     }
-    bool ok = true;
-    while (ok && ahead > 0) {
-#pragma unroll
-      for (int d = 0; d < XD; ++d) {
-        if (!ok || ahead == 0) break;
-        ok = store(buf[d]);
-        --ahead;
-        if (ok && more) {
-          load(buf[d]);
-          ++ahead;
-          more = advance();
-        }
-      }
-    }
+    cp_async_wait<0>();
   } else if (warp < kWarpT) {
     // ---------------- epilogue: base + accumulators -> y ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
+    constexpr int B = kEpiRows, RB = 64 * sizeof(YT);     // bytes of a row in the ring: this warp's 64 channels
+    const int nb = p.epi_ring / (B * RB);                 // batches: 1 to 4
     const YT* base = static_cast<const YT*>(p.a.base);
     YT* y = static_cast<YT*>(p.a.y);
-    const int quarter = warp & 3, half = (warp - kWarpEpi) >> 2, n_out = p.bank.n_out;
-    int32_t* rows = s_row + (warp - kWarpEpi) * 32;
-    uint32_t d = 0;
+    const int quarter = warp & 3, n_out = p.bank.n_out;
+    const uint32_t ring = smem_u32(sE) + (warp - kWarpEpi) * p.epi_ring;
+    // this warp's rows [i0, i1) of a unit: a fourth of them, eight at least
+    const int per = max(B, p.rt / 4), i0 = ((warp - kWarpEpi) >> 2) * per;
+    // the cursor of the copies: unit fu, chunk fc of [.., fc1), rows from fi. The rows follow each other from frow0
+    // (that of row i0), or lane i holds row i0 + i.
+    int64_t fu = blockIdx.x;
+    int fc = 0, fc1 = 0, fi = 0, fi1 = 0, frow0 = 0, frow = 0;
+    uint32_t fslot = ring;
+    auto open = [&]() -> bool {
+      for (; fu < n_units; fu += gridDim.x) {
+        const Unit un = get_unit(p, n_tiles, fu);
+        fi1 = min(un.rows, i0 + per);
+        if (un.ad.rank == 0 || i0 >= fi1) continue;
+        frow0 = un.row0 < 0 ? -1 : un.row0 + i0;
+        if (frow0 < 0) frow = p.plan.pos_row[un.pos0 + min(i0 + lane, fi1 - 1)];
+        fc = un.c0, fc1 = un.c1, fi = i0;
+        return true;
+      }
+      return false;
+    };
+    bool more = base && open();
+    auto fill = [&]() {  // the cursor's batch, one group (an empty one at the end)
+      if (more) {
+        const int ch = fc * 256 + quarter * 64, in = min(64, n_out - ch);  // channels of this warp's there are
+        // rows behind the unit's last one read it again
+        auto row_of = [&](int r) -> int64_t {
+          return frow0 >= 0 ? (int64_t)frow0 + min(fi + r, fi1 - 1) - i0
+                            : (int64_t)__shfl_sync(0xffffffffu, frow, fi - i0 + r);
+        };
+        if (p.b_copy == 16) {
+          constexpr int LPR = RB / 16, E16 = 16 / sizeof(YT), RPI = 32 / LPR;  // lanes per row, rows per instruction
+          const int c = lane % LPR * E16, bytes = max(0, min(16, (in - c) * (int)sizeof(YT)));
+          const uint32_t dst = fslot + lane / LPR * RB + c * sizeof(YT);
+          const YT* col = base + (bytes ? ch + c : 0);
+          if (frow0 >= 0 && fi + B <= fi1) {
+            const YT* src = col + (int64_t)(frow0 + fi - i0 + lane / LPR) * p.a.ldb;
+#pragma unroll
+            for (int j = 0; j < B; j += RPI, src += RPI * p.a.ldb) copy16(dst + j * RB, src, bytes);
+          } else {
+#pragma unroll
+            for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + row_of(j + lane / LPR) * p.a.ldb, bytes);
+          }
+        } else if (p.b_copy == 4) {
+          constexpr int E4 = 4 / sizeof(YT);
+#pragma unroll 2
+          for (int r = 0; r < B; ++r) {
+            const YT* src = base + row_of(r) * p.a.ldb;
+#pragma unroll
+            for (int c = lane * E4; c < 64; c += 32 * E4) {
+              const int bytes = max(0, min(4, (in - c) * (int)sizeof(YT)));
+              copy4(fslot + r * RB + c * sizeof(YT), src + (bytes ? ch + c : 0), bytes);
+            }
+          }
+        } else if constexpr (sizeof(YT) == 2) {  // odd 16-bit addresses: loads, clamped instead of conditional
+          const YT* c0 = base + min(ch + lane, n_out - 1);
+          const YT* c1 = base + min(ch + lane + 32, n_out - 1);
+          YT v0[B], v1[B];
+#pragma unroll
+          for (int r = 0; r < B; ++r) {
+            const int64_t o = row_of(r) * p.a.ldb;
+            v0[r] = c0[o], v1[r] = c1[o];
+          }
+          YT* dst = reinterpret_cast<YT*>(sE + (fslot - smem_u32(sE)));
+#pragma unroll
+          for (int r = 0; r < B; ++r) dst[r * 64 + lane] = v0[r], dst[r * 64 + lane + 32] = v1[r];
+        }
+        fslot += B * RB;
+        if (fslot == ring + p.epi_ring) fslot = ring;
+        fi += B;
+        if (fi >= fi1) {
+          fi = i0;
+          if (++fc == fc1) {
+            fu += gridDim.x;
+            more = open();
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    for (int b = 0; b < nb; ++b) fill();
+    uint32_t d = 0, slot = ring;
     bool ok = true;
     for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
       const Unit un = get_unit(p, n_tiles, u);
       if (un.rows <= 0) continue;
-      if (un.ad.rank == 0 && p.a.base == p.a.y && p.a.ldb == p.a.ldy) continue;  // in place, nothing to add
       if (un.ad.rank == 0) {
+        if (p.a.base == p.a.y && p.a.ldb == p.a.ldy) continue;  // in place, nothing to add
         const int cols = min(n_out, un.c1 * 256) - un.c0 * 256;
         for (int r = warp - kWarpEpi; r < un.rows; r += kEpiWarps) {
           const int64_t row = p.plan.pos_row[un.pos0 + r];
@@ -517,36 +537,69 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         }
         continue;
       }
-      // this warp's rows: a half of the unit's (rt = 16: the first half takes all)
-      const int i0 = p.rt >= 32 ? half * (p.rt / 2) : half * 16, i1 = min(un.rows, i0 + (p.rt >= 32 ? p.rt / 2 : 16));
-      __syncwarp();
-      if (i0 < i1) rows[lane] = p.plan.pos_row[un.pos0 + min(i0 + lane, i1 - 1)];
-      __syncwarp();
-      for (int c = un.c0; ok && c < un.c1; ++c, ++d) {
-        const int ch = c * 256 + quarter * 64 + lane * 2;
-        if (base && c + 1 < un.c1 && i0 + lane < i1) {  // the next chunk's lines of a row into L2
-          const YT* nb = base + (int64_t)rows[lane] * p.a.ldb;
-          prefetch_l2(nb + min(ch - lane * 2 + 256, n_out - 1));
-          if (sizeof(YT) == 4) prefetch_l2(nb + min(ch - lane * 2 + 288, n_out - 1));
-        }
-        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (d & 1) * 128u;
-        auto wait = [&]() -> bool {
-          ok = warp_wait(&dfull[d & 1], (d >> 1) & 1, abort_flag, err, 2u);
-          if (ok) tc_fence_after();
-          return ok;
-        };
-        if (p.y_vec)
-          epilogue_rows<YT, 2>(base, y, rows, p.a.ldb, p.a.ldy, ch, n_out, i0, i1, acc, p.rt, wait);
-        else
-          epilogue_rows<YT, 1>(base, y, rows, p.a.ldb, p.a.ldy, ch, n_out, i0, i1, acc, p.rt, wait);
+      const int i1 = min(un.rows, i0 + per);
+      const int my_row = un.row0 < 0 && i0 < i1 ? p.plan.pos_row[un.pos0 + min(i0 + lane, i1 - 1)] : 0;
+      for (int c = un.c0; c < un.c1; ++c, ++d) {
+        ok = warp_wait(&dfull[d & 1], (d >> 1) & 1, abort_flag, err, 2u);
         if (!ok) break;
+        tc_fence_after();
+        const int ch = c * 256 + quarter * 64 + lane * 2;
+        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (d & 1) * 128u;
+        for (int i = i0; i < i1; i += B) {
+          Pair b[B];
+          if (base) {
+            copy_wait(nb - 1);
+            __syncwarp();
+            const uint8_t* src = sE + (slot - smem_u32(sE)) + lane * 2 * sizeof(YT);
+#pragma unroll
+            for (int j = 0; j < B; ++j) b[j] = *reinterpret_cast<const Pair*>(src + j * RB);
+            slot += B * RB;
+            if (slot == ring + p.epi_ring) slot = ring;
+            __syncwarp();
+            fill();
+          } else {
+#pragma unroll
+            for (int j = 0; j < B; ++j) b[j].e[0] = b[j].e[1] = as_type<YT>(0.0f);
+          }
+          uint32_t v0[B], v1[B];
+          tmem_ld8(acc + (uint32_t)i, v0);
+          tmem_ld8(acc + (uint32_t)(p.rt + i), v1);
+          tmem_wait_ld();
+          reg_barrier8(v0);
+          reg_barrier8(v1);
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            b[j].e[0] = as_type<YT>(__fadd_rn(as_f32(b[j].e[0]), __uint_as_float(v0[j])));
+            b[j].e[1] = as_type<YT>(__fadd_rn(as_f32(b[j].e[1]), __uint_as_float(v1[j])));
+          }
+          if (p.y_pair && un.row0 >= 0 && i + B <= i1) {  // the usual case in few instructions
+            if (ch < n_out) {
+              YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + ch;
+#pragma unroll
+              for (int j = 0; j < B; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+              const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
+              if (i + j >= i1) continue;
+              YT* dst = y + (int64_t)row * p.a.ldy + ch;
+              if (p.y_pair) {
+                if (ch < n_out) *reinterpret_cast<Pair*>(dst) = b[j];
+              } else {
+                if (ch < n_out) dst[0] = b[j].e[0];
+                if (ch + 1 < n_out) dst[1] = b[j].e[1];
+              }
+            }
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&dempty[d & 1]);
       }
     }
+    cp_async_wait<0>();
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp < kWarpShrink) {
     // ---------------- t: TMEM -> scaled, split -> shared memory ----------------
     const int quarter = warp & 3, row = quarter * 32 + lane;  // this lane's row of the unit
@@ -623,28 +676,38 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         tc_fence_after();
         const uint32_t acc0 = tmem + set * 128u, acc_lo = acc0 + (uint32_t)(sa.hi_parts * sa.width);
         int c = 0;
+        uint32_t more_lo = 0;
         for (int part = 0; ok && part < sa.hi_parts; ++part) {
           const uint32_t acc = acc0 + (uint32_t)(part * sa.width);
           const int end = k_stages * (part + 1) / sa.hi_parts;
           for (uint32_t more = 0; c < end; ++c) {
-            ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u) &&
-                 stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
-            if (!ok) break;
+            ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u);
             tc_fence_after();
-            const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot), w0 = desc_lo(smem_u32(sA) + ar.slot * a_slot);
-            const uint32_t lo_x = x_atom >> 3, lo_w = a_rows << 4;  // from the hi to the lo plane
+            const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot);
+            for (int pl = 0; pl < PW; ++pl) {
+              for (int at = 0; at < 2; ++at) {
+                ok = ok && stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t x = x0 + at * (x_atom >> 4), w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
 #pragma unroll
-            for (int s = 0; s < KS / 8; ++s) {
-              const uint32_t x = x0 + s / 4 * (x_atom >> 4) + s % 4 * 2, w = w0 + s / 4 * (a_rows << 3) + s % 4 * 2;
-              umma_tf32(acc, desc_at(x), desc_at(w), id, s > 0 ? 1 : more);
-              if (PX == 2) umma_tf32(acc_lo, desc_at(x + lo_x), desc_at(w), id, c > 0 || s > 0);
-              if (PW == 2) umma_tf32(acc_lo, desc_at(x), desc_at(w + lo_w), id, PX == 2 || c > 0 || s > 0);
+                for (int s = 0; s < KC / 8; ++s) {
+                  if (pl == 0) {
+                    umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, more);
+                    more = 1;
+                    if (PX == 2) umma_tf32(acc_lo, desc_at(x + (x_atom >> 3) + 2 * s), desc_at(w + 2 * s), id, more_lo);
+                  } else {
+                    umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, more_lo);
+                  }
+                  if (PX == 2 || pl > 0) more_lo = 1;
+                }
+                umma_commit(&aempty[ar.slot]);
+                ar.next(p.a_slots);
+              }
             }
-            more = 1;
+            if (!ok) break;
             umma_commit(&xempty[xr.slot]);
-            umma_commit(&aempty[ar.slot]);
             xr.next(p.x_slots);
-            ar.next(p.a_slots);
           }
         }
         if (ok) umma_commit(&tafull[set]);
@@ -673,20 +736,23 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             const uint32_t acc = tmem + 256u + (d & 1) * 128u + (uint32_t)(g * p.rt);
             uint32_t t = desc_lo(smem_u32(sT) + tr.slot * t_buf), more = 0;
             for (int left = un.ad.rp / 8; ok && left > 0; left -= KC / 8) {
-              ok = stage_wait(&bfull[br.slot], br.parity, abort_flag, err, 1024u);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t w = desc_lo(smem_u32(sB) + br.slot * b_slot);
+              for (int pl = 0; pl < PW; ++pl) {
+                ok = ok && stage_wait(&bfull[br.slot], br.parity, abort_flag, err, 1024u);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t w = desc_lo(smem_u32(sB) + br.slot * kBPlane);
 #pragma unroll
-              for (int s = 0; s < KC / 8; ++s) {
-                if (s >= left) break;
-                umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + (t_plane >> 4) + 2 * s), id, s > 0 ? 1 : more);
-                if (PW == 2) umma_tf32(acc, desc_at(w + (kBPlane >> 4) + 2 * s), desc_at(t + 2 * s), id, 1);
-                umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + 2 * s), id, 1);
+                for (int s = 0; s < KC / 8; ++s) {
+                  if (s >= left) break;
+                  if (pl == 0) {
+                    umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + (t_plane >> 4) + 2 * s), id, more);
+                    more = 1;
+                  }
+                  umma_tf32(acc, desc_at(w + 2 * s), desc_at(t + 2 * s), id, 1);
+                }
+                umma_commit(&bempty[br.slot]);
+                br.next(p.b_slots);
               }
-              more = 1;
-              umma_commit(&bempty[br.slot]);
-              br.next(p.b_slots);
               t += 2 * t_plane >> 4;
             }
           }
@@ -702,8 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     // ---------------- weights: bulk copies of the bank's tiles (A's, or B's) ----------------
     const bool is_a = warp == kWarpA;
     uint8_t* ring = is_a ? sA : sB;
-    const uint32_t slots = is_a ? p.a_slots : p.b_slots, slot = is_a ? a_slot : b_slot;
-    const uint32_t pieces = is_a ? 2 * PW : PW, to_piece = is_a ? a_rows * 128 : kBPlane;  // per slot
+    const uint32_t slots = is_a ? p.a_slots : p.b_slots, slot = is_a ? a_slot : kBPlane;
     uint64_t *full = is_a ? afull : bfull, *empty = is_a ? aempty : bempty;
     Ring r;
     uint32_t issued = 0;
@@ -714,12 +779,11 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int rcs = (un.ad.rp + KC - 1) / KC;
       const uint32_t bytes = is_a ? un.ad.rank * 128 : kBPlane;  // of a piece
       const uint8_t* src = is_a ? un.ad.ta : un.ad.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
-      for (int n = is_a ? k_stages : (un.c1 - un.c0) * 2 * rcs; n > 0; --n) {
+      for (int n = is_a ? k_stages * 2 * PW : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
         ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
         if (!ok) break;
-        mbar_arrive_expect_tx(&full[r.slot], bytes * pieces);
-        for (uint32_t i = 0; i < pieces; ++i, src += bytes)
-          bulk_load(ring + r.slot * slot + i * to_piece, src, bytes, &full[r.slot]);
+        mbar_arrive_expect_tx(&full[r.slot], bytes);
+        bulk_load(ring + r.slot * slot, src, bytes, &full[r.slot]);
         r.next(slots);
         ++issued;
       }
@@ -783,7 +847,6 @@ __global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int
 template <class XT, class YT>
 cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;
-  const int planes = p.bank.wtype == kDtF32 ? 2 : 1;
   const int chunks = (p.bank.n_out + 255) / 256;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -793,26 +856,37 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   p.splits = 1;
   while (p.rt > 16 && (int64_t)n_tiles * (kAdapterTileRows / p.rt) < sms) p.rt /= 2;
   while (p.splits < chunks && (int64_t)n_tiles * (kAdapterTileRows / p.rt) * (p.splits + 1) <= sms) ++p.splits;
-  // Shared memory: rings of two to four slots, and a second buffer of t when there is room.
-  const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = planes * 2 * ((p.bank.max_rank + 15) / 16 * 16) * 128;
+  // Shared memory: the most rows that fit two slots of every ring, then what is left for more of them.
+  const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = (p.bank.max_rank + 15) / 16 * 16 * 128;
   int smem = 0;
-  for (;; p.rt /= 2) {
+  for (; p.rt >= 16; p.rt /= 2) {
     const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * 2 * p.rt * 128;
-    int left = kMaxSmem - 1024 - kMiscBytes - 2 * (planes * kBPlane + a_slot + x_slot) - t_buf;
+    int left = kMaxSmem - 1024 - kMiscBytes - kEpiWarps * 2048 - 2 * (kBPlane + a_slot + x_slot) - t_buf;
     if (left < 0) continue;
-    p.t_bufs = 1, p.a_slots = p.b_slots = p.x_slots = 2;
-    for (int round = 0; round < 2; ++round) {
-      if (left >= x_slot) left -= x_slot, ++p.x_slots;
-      if (round == 0 && left >= t_buf) left -= t_buf, ++p.t_bufs;
-      if (left >= a_slot) left -= a_slot, ++p.a_slots;
-      if (left >= planes * kBPlane) left -= planes * kBPlane, ++p.b_slots;
+    p.t_bufs = 1, p.a_slots = p.b_slots = p.x_slots = 2, p.epi_ring = 2048;
+    auto grow = [&](int32_t& n, int by, int most, int bytes) {
+      if (n + by > most || left < bytes) return false;
+      left -= bytes, n += by;
+      return true;
+    };
+    grow(p.x_slots, 1, 3, x_slot);
+    grow(p.epi_ring, 2048, 4096, kEpiWarps * 2048);
+    for (bool any = true; any;) {
+      any = grow(p.b_slots, 1, kMaxSlots, kBPlane);
+      any |= grow(p.a_slots, 1, kMaxSlots, a_slot);
+      any |= grow(p.x_slots, 1, 6, x_slot);
+      any |= grow(p.t_bufs, 1, 2, t_buf);
     }
     smem = kMaxSmem - left;
     break;
   }
+  if (!smem) return cudaErrorInvalidValue;
   p.x_vec = (reinterpret_cast<uintptr_t>(p.a.x) & 15) == 0 && (p.a.ldx * sizeof(XT)) % 16 == 0;
-  p.y_vec = p.bank.n_out % 2 == 0 && p.a.ldy % 2 == 0 && (!p.a.base || p.a.ldb % 2 == 0) &&
-            ((reinterpret_cast<uintptr_t>(p.a.y) | reinterpret_cast<uintptr_t>(p.a.base)) & (2 * sizeof(YT) - 1)) == 0;
+  const uintptr_t base = reinterpret_cast<uintptr_t>(p.a.base);
+  p.b_copy = (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 16 == 0 ? 16
+             : (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 4 == 0 ? 4 : 2;
+  p.y_pair = p.bank.n_out % 2 == 0 &&
+             (reinterpret_cast<uintptr_t>(p.a.y) | (uint64_t)(p.a.ldy * sizeof(YT))) % (2 * sizeof(YT)) == 0;
   e = cudaFuncSetAttribute(lowrank_tc_kernel<XT, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;

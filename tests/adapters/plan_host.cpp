@@ -12,7 +12,7 @@ const char* ph_check(const int32_t* offsets, const int32_t* adapters, int32_t n_
   return why ? why : "";
 }
 
-// tiles: room for max_large + max_small of {adapter, pos0, rows}; order: n_seqs,
+// tiles: room for max_large + max_small of {adapter, pos0, rows, row0}; order: n_seqs,
 // pos: n_seqs + 1. counts: large, small, rows, max adapter.
 void ph_build(const int32_t* offsets, const int32_t* adapters, int32_t n_seqs, int32_t* order, int32_t* pos,
               int32_t* large, int32_t* small, int32_t* counts) {

@@ -59,7 +59,7 @@ def _check_plan(lib, lengths, adapters):
     n, rows = len(lengths), int(offs[-1])
     cap = lib.ph_max_large(rows, n)
     order, pos = np.full(n, -9, np.int32), np.full(n + 1, -9, np.int32)
-    large, small = np.zeros((cap + 1, 3), np.int32), np.zeros((n + 1, 3), np.int32)
+    large, small = np.zeros((cap + 1, 4), np.int32), np.zeros((n + 1, 4), np.int32)
     counts = np.zeros(4, np.int32)
     lib.ph_build(offs.ctypes.data, ad.ctypes.data, n, order.ctypes.data, pos.ctypes.data, large.ctypes.data,
                  small.ctypes.data, counts.ctypes.data)
@@ -72,10 +72,11 @@ def _check_plan(lib, lengths, adapters):
     adapter_of = np.repeat(ad, lengths) if n else np.zeros(0, int)
     seen = np.zeros(rows, int)
     for tiles, most in ((large[:counts[0]], lib.ph_tile_rows()), (small[:counts[1]], lib.ph_small_rows())):
-        for a, p0, r in tiles:
+        for a, p0, r, first in tiles:
             assert 0 < r <= most and 0 <= p0 and p0 + r <= rows
             at = row_at[p0:p0 + r]
             assert (adapter_of[at] == a).all()
+            assert first == (at[0] if (np.diff(at) == 1).all() else -1)
             seen[at] += 1
     assert (seen == 1).all()
     for i, s in enumerate(order):
