@@ -48,7 +48,11 @@ constexpr int kXWarps = 8, kEpiWarps = 16, kTWarps = 2;
 constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
 constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1;
 constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA and copy warps, two idle
-static_assert(kThreads == 1024, "64 registers each");
+// Registers: 1024 threads get 64 each at launch; the last two warpgroups give
+// some back (setmaxnreg) to the x and the epilogue warpgroups, which would
+// spill otherwise, into an L1 that the shared memory leaves too small for it.
+constexpr int kRegsX = 72, kRegsEpi = 72, kRegsRest = 40;
+static_assert(kThreads == 1024 && kXWarps * kRegsX + kEpiWarps * kRegsEpi + 8 * kRegsRest <= 32 * 64, "register split");
 static_assert(kWarpEpi % 4 == 0 && kWarpT % 4 == 0, "TMEM lane quarters go by warp index");
 constexpr int KC = 32;   // tf32 per swizzled 128-byte row
 constexpr int KS = 64;   // input channels per stage: two such rows
@@ -322,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 
   if (warp < kXWarps) {
     // ---------------- x: global -> swizzled shared memory, split in place ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsX));
     const int k = p.bank.k_in;
     const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
     const int full_stages = p.x_vec ? k / KS : 0;  // stages that 16-byte copies can take
@@ -435,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     cp_async_wait<0>();
   } else if (warp < kWarpT) {
     // ---------------- epilogue: base + accumulators -> y ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
     constexpr int B = kEpiRows, RB = 64 * sizeof(YT);     // bytes of a row in the ring: this warp's 64 channels
     const int nb = p.epi_ring / (B * RB);                 // batches: 1 to 4
@@ -600,6 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     }
     cp_async_wait<0>();
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp < kWarpShrink) {
     // ---------------- t: TMEM -> scaled, split -> shared memory ----------------
     const int quarter = warp & 3, row = quarter * 32 + lane;  // this lane's row of the unit
@@ -676,7 +683,6 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         tc_fence_after();
         const uint32_t acc0 = tmem + set * 128u, acc_lo = acc0 + (uint32_t)(sa.hi_parts * sa.width);
         int c = 0;
-        uint32_t more_lo = 0;
         for (int part = 0; ok && part < sa.hi_parts; ++part) {
           const uint32_t acc = acc0 + (uint32_t)(part * sa.width);
           const int end = k_stages * (part + 1) / sa.hi_parts;
@@ -684,27 +690,36 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u);
             tc_fence_after();
             const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot);
-            for (int pl = 0; pl < PW; ++pl) {
-              for (int at = 0; at < 2; ++at) {
-                ok = ok && stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t x = x0 + at * (x_atom >> 4), w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
+            // a piece of A (32 channels of a plane) against the planes of x
+            auto piece = [&](int at, bool low) {
+              if (!ok) return;
+              ok = stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
+              if (!ok) return;
+              tc_fence_after();
+              const uint32_t x = x0 + at * (x_atom >> 4), w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
+              if (!low) {
 #pragma unroll
                 for (int s = 0; s < KC / 8; ++s) {
-                  if (pl == 0) {
-                    umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, more);
-                    more = 1;
-                    if (PX == 2) umma_tf32(acc_lo, desc_at(x + (x_atom >> 3) + 2 * s), desc_at(w + 2 * s), id, more_lo);
-                  } else {
-                    umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, more_lo);
-                  }
-                  if (PX == 2 || pl > 0) more_lo = 1;
+                  umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, s > 0 || at > 0 ? 1 : more);
+                  if (PX == 2)
+                    umma_tf32(acc_lo, desc_at(x + (x_atom >> 3) + 2 * s), desc_at(w + 2 * s), id,
+                              s > 0 || at > 0 ? 1 : c > 0);
                 }
-                umma_commit(&aempty[ar.slot]);
-                ar.next(p.a_slots);
+              } else {
+#pragma unroll
+                for (int s = 0; s < KC / 8; ++s)
+                  umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, PX == 2 || s > 0 || at > 0 ? 1 : c > 0);
               }
+              umma_commit(&aempty[ar.slot]);
+              ar.next(p.a_slots);
+            };
+            piece(0, false);
+            piece(1, false);
+            if (PW == 2) {
+              piece(0, true);
+              piece(1, true);
             }
+            more = 1;
             if (!ok) break;
             umma_commit(&xempty[xr.slot]);
             xr.next(p.x_slots);
