@@ -27,6 +27,7 @@
 //   - a shrink and an expand MMA thread, so that the shrink of later units
 //     goes on while the epilogue holds up the expand of an earlier one;
 //   - T warps (2): t from TMEM, scaled, split, to shared memory;
+//   - a unit warp: what to do next, looked up ahead for all the others;
 //   - epilogue warps (16): base by asynchronous copies into a ring per warp,
 //     ahead of the accumulators and across units.
 // One persistent CTA per SM. Loads into registers in place of the asynchronous
@@ -46,8 +47,8 @@ namespace {
 
 constexpr int kXWarps = 8, kEpiWarps = 16, kTWarps = 2;
 constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
-constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1;
-constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA and copy warps, two idle
+constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1, kWarpUnits = kWarpB + 1;
+constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA, copy and unit warps, one idle
 // Registers: 1024 threads get 64 each at launch; the last two warpgroups give
 // some back (setmaxnreg) to the x and the epilogue warpgroups, which would
 // spill otherwise, into an L1 that the shared memory leaves too small for it.
@@ -60,7 +61,7 @@ constexpr int kRt = 64;  // rows per unit at most
 static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile or a part of one");
 constexpr int kMaxSlots = 8;
 constexpr int kBPlane = 128 * 128;  // one plane of a slot of B: 128 channels x 128 bytes
-constexpr int kMiscBytes = 512;
+constexpr int kMiscBytes = 1280;
 constexpr int kEpiRows = 8;  // rows per batch of an epilogue warp's ring of base
 constexpr int kMaxSmem = 232448;  // an MMA reads 128 rows from a slot's start: a short slot's run on into sW and sT
 
@@ -216,12 +217,20 @@ struct ShrinkAcc {
   }
 };
 
-struct Unit {
-  LowRankAdapter ad;
-  int32_t pos0, rows;  // positions; rows <= 0: nothing
+// What a CTA does next. The unit warp looks it up (32 units at a time, so that
+// the dependent loads of tile and adapter cost no role anything) and passes it
+// on through a ring in shared memory; the last entry has no rows.
+struct alignas(16) Unit {
+  const uint8_t* ta;
+  const uint8_t* tb;
+  int32_t pos0, rows;  // positions
   int32_t row0;        // their rows follow each other from here, or -1
   int32_t c0, c1;      // chunks of 256 output channels
+  int32_t rank, rp;    // rank 0: y = base
+  float scale;
 };
+constexpr int kUnitSlots = 8;  // above the four units that an epilogue warp's copies can be ahead of its stores
+constexpr int kUnitReaders = kXWarps + kEpiWarps + kTWarps + 4;
 
 struct TcParams {
   LowRankBank bank;
@@ -236,8 +245,8 @@ struct TcParams {
   uint32_t* err;
 };
 
-// Unit u: sub-tiles of the same number lie together, so that those behind a
-// tile's last row (they are skipped) come last.
+// Unit u. Sub-tiles of the same number lie together, so that those behind a
+// tile's last row come last.
 __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t u) {
   Unit r;
   const int split = (int)(u % p.splits);
@@ -250,11 +259,36 @@ __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t
   const int chunks = (p.bank.n_out + 255) / 256;
   r.c0 = chunks * split / p.splits;
   r.c1 = chunks * (split + 1) / p.splits;
-  r.ad = LowRankAdapter{};
-  if (r.rows > 0 && r.c1 > r.c0 && tl.adapter >= 0 && tl.adapter < p.bank.n_adapters)
-    r.ad = p.bank.adapters[tl.adapter];
+  r.ta = r.tb = nullptr;
+  r.rank = r.rp = 0;
+  r.scale = 0.0f;
+  if (r.rows > 0 && tl.adapter >= 0 && tl.adapter < p.bank.n_adapters) {
+    const LowRankAdapter ad = p.bank.adapters[tl.adapter];
+    r.ta = ad.ta, r.tb = ad.tb, r.rank = ad.rank, r.rp = ad.rp, r.scale = ad.scale;
+  }
   return r;
 }
+
+// A role's position in the ring of units.
+struct UnitCursor {
+  Ring r;
+  // The next unit into `un`; false at the end or when the kernel gives up. Called by a whole warp (WARP) or by one
+  // thread of it. RELEASE: the entry is free as far as this reader goes.
+  template <bool WARP, bool RELEASE>
+  __device__ __forceinline__ bool next(Unit& un, const Unit* units, uint64_t* full, uint64_t* empty,
+                                       volatile int* abort_flag, uint32_t* err) {
+    const bool ok = WARP ? warp_wait(&full[r.slot], r.parity, abort_flag, err, 4096u)
+                         : stage_wait(&full[r.slot], r.parity, abort_flag, err, 4096u);
+    if (!ok) return false;
+    un = units[r.slot];
+    if (RELEASE) {
+      if (WARP) __syncwarp();
+      if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&empty[r.slot]);
+    }
+    r.next(kUnitSlots);
+    return un.rows > 0;
+  }
+};
 
 template <class XT, class YT>
 __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_constant__ TcParams p) {
@@ -289,8 +323,12 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   uint64_t* dfull = tfree + 2;            // an expand accumulator is complete / read
   uint64_t* dempty = dfull + 2;
   uint64_t* drain = dempty + 2;           // [2] the MMA threads' last MMAs
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
+  uint64_t* ufull = drain + 2;            // the ring of units
+  uint64_t* uempty = ufull + kUnitSlots;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(uempty + kUnitSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
+  Unit* units = reinterpret_cast<Unit*>(misc + 768);
+  static_assert((6 * kMaxSlots + 14 + 2 * kUnitSlots) * 8 + 8 <= 768 && 768 + sizeof(Unit) * kUnitSlots <= kMiscBytes, "");
   uint32_t* err = p.err ? p.err : &g_lowrank_error;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -312,6 +350,10 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       mbar_init(&tfree[i], 1);
       mbar_init(&drain[i], 1);
     }
+    for (int i = 0; i < kUnitSlots; ++i) {
+      mbar_init(&ufull[i], 1);
+      mbar_init(&uempty[i], kUnitReaders);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -320,8 +362,6 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;  // shrink accumulators at columns 0 and 128, expand at 256 and 384
-  const int n_tiles = p.plan.counts[0];
-  const int64_t n_units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
   const int k_stages = p.bank.ka / KS;
 
   if (warp < kXWarps) {
@@ -331,25 +371,23 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
     const int full_stages = p.x_vec ? k / KS : 0;  // stages that 16-byte copies can take
     const XT* row[XV];
-    // the cursor of the copies: unit u, its stage ks
-    int64_t u = blockIdx.x;
+    // the cursor of the copies: a unit, its stage ks
+    UnitCursor uc;
     int ks = 0, passes = 0;
-    auto open = [&]() -> bool {  // the next unit with something to add from u on
-      for (; u < n_units; u += gridDim.x) {
-        const Unit un = get_unit(p, n_tiles, u);
-        if (un.rows <= 0 || un.ad.rank == 0) continue;
-        passes = (un.rows + XR - 1) / XR;  // later ones have no rows
+    auto open = [&]() -> bool {  // the next unit with something to add
+      Unit un;
+      do {
+        if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) return false;
+      } while (un.rank == 0);
+      passes = (un.rows + XR - 1) / XR;  // later ones have no rows
 #pragma unroll
-        for (int i = 0; i < XV; ++i)  // behind the last row: that row again
-        {
-          const int r = min(r0 + i * XR, un.rows - 1);
-          row[i] = static_cast<const XT*>(p.a.x) +
-                   (int64_t)(un.row0 >= 0 ? un.row0 + r : p.plan.pos_row[un.pos0 + r]) * p.a.ldx;
-        }
-        ks = 0;
-        return true;
+      for (int i = 0; i < XV; ++i) {  // behind the last row: that row again
+        const int r = min(r0 + i * XR, un.rows - 1);
+        row[i] = static_cast<const XT*>(p.a.x) +
+                 (int64_t)(un.row0 >= 0 ? un.row0 + r : p.plan.pos_row[un.pos0 + r]) * p.a.ldx + col;
       }
-      return false;
+      ks = 0;
+      return true;
     };
     // This thread's 16-byte pieces of its first row in a slot (its other rows are multiples of 8 further). A copy
     // of 16-bit values lands where the first or, in lanes of the upper 32 channels, the second of its two pieces
@@ -371,11 +409,11 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         for (int i = 0; i < XV; ++i) {
           if (i >= passes || r0 + i * XR >= p.rt) break;
           if (ks < full_stages) {
-            copy16(smem_u32(dst) + i * XR * 128, row[i] + c, 16);
+            copy16(smem_u32(dst) + i * XR * 128, row[i] + ks * KS, 16);
           } else {
             XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
 #pragma unroll
-            for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1)];
+            for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1) - col];
             uint32_t v[4];
             if constexpr (PX == 2) {
 #pragma unroll
@@ -391,10 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         }
         ir.next(p.x_slots);
         ++pending;
-        if (++ks == k_stages) {
-          u += gridDim.x;
-          more = open();
-        }
+        if (++ks == k_stages) more = open();
       }
       cp_async_commit();
     };
@@ -450,16 +485,24 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     const uint32_t ring = smem_u32(sE) + (warp - kWarpEpi) * p.epi_ring;
     // this warp's rows [i0, i1) of a unit: a fourth of them, eight at least
     const int per = max(B, p.rt / 4), i0 = ((warp - kWarpEpi) >> 2) * per;
-    // the cursor of the copies: unit fu, chunk fc of [.., fc1), rows from fi. The rows follow each other from frow0
+    // the cursor of the copies: a unit, chunk fc of [.., fc1), rows from fi. The rows follow each other from frow0
     // (that of row i0), or lane i holds row i0 + i.
-    int64_t fu = blockIdx.x;
+    UnitCursor fu, uc;
     int fc = 0, fc1 = 0, fi = 0, fi1 = 0, frow0 = 0, frow = 0;
     uint32_t fslot = ring;
+    int ahead = 0;    // units that fu is ahead of uc: the ring holds kUnitSlots, and uc alone frees them
+    int filled = 0;   // batches copied and not yet used
+    bool more = false, end = base == nullptr;
     auto open = [&]() -> bool {
-      for (; fu < n_units; fu += gridDim.x) {
-        const Unit un = get_unit(p, n_tiles, fu);
+      while (!end && ahead < kUnitSlots - 2) {
+        Unit un;
+        if (!fu.next<true, false>(un, units, ufull, uempty, abort_flag, err)) {
+          end = true;
+          break;
+        }
+        ++ahead;
         fi1 = min(un.rows, i0 + per);
-        if (un.ad.rank == 0 || i0 >= fi1) continue;
+        if (un.rank == 0 || i0 >= fi1) continue;
         frow0 = un.row0 < 0 ? -1 : un.row0 + i0;
         if (frow0 < 0) frow = p.plan.pos_row[un.pos0 + min(i0 + lane, fi1 - 1)];
         fc = un.c0, fc1 = un.c1, fi = i0;
@@ -467,8 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       }
       return false;
     };
-    bool more = base && open();
-    auto fill = [&]() {  // the cursor's batch, one group (an empty one at the end)
+    auto fill = [&]() {  // the cursor's batch, if there is one, as one group of copies
+      if (!more) more = open();
       if (more) {
         const int ch = fc * 256 + quarter * 64, in = min(64, n_out - ch);  // channels of this warp's there are
         // rows behind the unit's last one read it again
@@ -518,22 +561,21 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         fi += B;
         if (fi >= fi1) {
           fi = i0;
-          if (++fc == fc1) {
-            fu += gridDim.x;
-            more = open();
-          }
+          more = ++fc < fc1;
         }
+        cp_async_commit();
+        ++filled;
       }
-      cp_async_commit();
     };
     for (int b = 0; b < nb; ++b) fill();
     uint32_t d = 0, slot = ring;
     bool ok = true;
-    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-      const Unit un = get_unit(p, n_tiles, u);
-      if (un.rows <= 0) continue;
-      if (un.ad.rank == 0) {
-        if (p.a.base == p.a.y && p.a.ldb == p.a.ldy) continue;  // in place, nothing to add
+    Unit un;
+    while (ok) {
+      if (!more) more = open();  // fu reads an entry before uc frees it
+      if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) break;
+      --ahead;
+      if (un.rank == 0) {
         const int cols = min(n_out, un.c1 * 256) - un.c0 * 256;
         for (int r = warp - kWarpEpi; r < un.rows; r += kEpiWarps) {
           const int64_t row = p.plan.pos_row[un.pos0 + r];
@@ -554,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         for (int i = i0; i < i1; i += B) {
           Pair b[B];
           if (base) {
-            copy_wait(nb - 1);
+            if (!filled) fill();  // the cursor was at its limit
+            copy_wait(--filled);
             __syncwarp();
             const uint8_t* src = sE + (slot - smem_u32(sE)) + lane * 2 * sizeof(YT);
 #pragma unroll
@@ -613,21 +656,22 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     uint32_t q = 0;
     Ring tr;
     bool ok = true;
-    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-      const Unit un = get_unit(p, n_tiles, u);
-      if (un.rows <= 0 || un.ad.rank == 0) continue;
-      float sc = un.ad.scale;
+    UnitCursor uc;
+    Unit un;
+    while (ok && uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) {
+      if (un.rank == 0) continue;
+      float sc = un.scale;
       if (p.a.absmax && row < un.rows)
         sc = __fmul_rn(sc, __fdiv_rn(__uint_as_float(p.a.absmax[p.a.per_seq ? p.plan.pos_seq[un.pos0 + row] : 0]),
                                      127.0f));
-      const ShrinkAcc sa(p.bank.max_rank, un.ad.rank, PX == 2 || PW == 2, k_stages);
+      const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PW == 2, k_stages);
       ok = warp_wait(&tafull[(q & (sa.bufs - 1))], (q >> (sa.bufs - 1)) & 1, abort_flag, err, 4u) &&
            warp_wait(&tfree[tr.slot], tr.parity ^ 1, abort_flag, err, 8u);
       if (!ok) break;
       tc_fence_after();
       if (quarter * 32 < un.rows) {
         const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + ((q & (sa.bufs - 1))) * 128u;
-        for (int j = 0; j < un.ad.rp; j += 8) {  // eight ranks: two 16-byte pieces of each plane
+        for (int j = 0; j < un.rp; j += 8) {  // eight ranks: two 16-byte pieces of each plane
           float t[8];
           {
             uint32_t v[8];
@@ -648,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           float hi[8], lo[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)  // ranks behind the last one meet zero columns of B: they have to be finite
-            split_tf32(j + e < un.ad.rank ? __fmul_rn(t[e], sc) : 0.0f, hi[e], lo[e]);
+            split_tf32(j + e < un.rank ? __fmul_rn(t[e], sc) : 0.0f, hi[e], lo[e]);
           uint8_t* dst = sT + tr.slot * t_buf + (j / KC) * 2 * t_plane + row * 128;
           if (row >= p.rt) continue;  // lanes without a row of t (units of 16 rows)
           const int c0 = (j % KC) / 4, x = row & 7;
@@ -674,10 +718,11 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       Ring xr, ar;
       uint32_t q = 0;
       bool ok = true;
-      for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-        const Unit un = get_unit(p, n_tiles, u);
-        if (un.rows <= 0 || un.ad.rank == 0) continue;
-        const ShrinkAcc sa(p.bank.max_rank, un.ad.rank, PX == 2 || PW == 2, k_stages);
+      UnitCursor uc;
+      Unit un;
+      while (ok && uc.next<false, true>(un, units, ufull, uempty, abort_flag, err)) {
+        if (un.rank == 0) continue;
+        const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PW == 2, k_stages);
         const uint32_t set = q & (sa.bufs - 1), id = idesc_tf32(128, sa.width);
         ok = stage_wait(&taempty[set], ((q >> (sa.bufs - 1)) & 1) ^ 1, abort_flag, err, 16u);
         tc_fence_after();
@@ -739,9 +784,10 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       Ring br, tr;
       uint32_t d = 0;
       bool ok = true;
-      for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-        const Unit un = get_unit(p, n_tiles, u);
-        if (un.rows <= 0 || un.ad.rank == 0) continue;
+      UnitCursor uc;
+      Unit un;
+      while (ok && uc.next<false, true>(un, units, ufull, uempty, abort_flag, err)) {
+        if (un.rank == 0) continue;
         ok = stage_wait(&tfull[tr.slot], tr.parity, abort_flag, err, 128u);
         tc_fence_after();
         for (int c = un.c0; ok && c < un.c1; ++c, ++d) {
@@ -750,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           for (int g = 0; ok && g < 2; ++g) {  // even, then odd channels
             const uint32_t acc = tmem + 256u + (d & 1) * 128u + (uint32_t)(g * p.rt);
             uint32_t t = desc_lo(smem_u32(sT) + tr.slot * t_buf), more = 0;
-            for (int left = un.ad.rp / 8; ok && left > 0; left -= KC / 8) {
+            for (int left = un.rp / 8; ok && left > 0; left -= KC / 8) {
               for (int pl = 0; pl < PW; ++pl) {
                 ok = ok && stage_wait(&bfull[br.slot], br.parity, abort_flag, err, 1024u);
                 if (!ok) break;
@@ -779,6 +825,36 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       umma_commit(&drain[1]);
       mbar_wait_drain(&drain[1], 0);
     }
+  } else if (warp == kWarpUnits) {
+    // ---------------- units: looked up 32 at a time ----------------
+    const int n_tiles = p.plan.counts[0];
+    const int64_t n_units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
+    const bool in_place = p.a.base == p.a.y && p.a.ldb == p.a.ldy;  // nothing to do for rows without an adapter
+    Ring r;
+    bool ok = true;
+    for (int64_t first = blockIdx.x; ok; first += 32 * (int64_t)gridDim.x) {
+      const int64_t u = first + lane * (int64_t)gridDim.x;
+      Unit un;
+      un.rows = 0;
+      if (u < n_units) un = get_unit(p, n_tiles, u);
+      uint32_t todo = __ballot_sync(0xffffffffu, un.rows > 0 && un.c1 > un.c0 && (un.rank > 0 || !in_place));
+      const bool last = first + 32 * (int64_t)gridDim.x >= n_units;
+      while (ok && (todo || last)) {
+        const int from = todo ? __ffs(todo) - 1 : 0;  // without one left: the end, an entry without rows
+        ok = warp_wait(&uempty[r.slot], r.parity ^ 1, abort_flag, err, 8192u);
+        if (!ok) break;
+        if (lane == from) {
+          if (!todo) un.rows = 0;
+          units[r.slot] = un;
+          mbar_arrive(&ufull[r.slot]);
+        }
+        __syncwarp();
+        r.next(kUnitSlots);
+        if (!todo) break;
+        todo &= todo - 1;
+      }
+      if (last) break;
+    }
   } else if (warp <= kWarpB && lane == 0) {
     // ---------------- weights: bulk copies of the bank's tiles (A's, or B's) ----------------
     const bool is_a = warp == kWarpA;
@@ -788,12 +864,13 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     Ring r;
     uint32_t issued = 0;
     bool ok = true;
-    for (int64_t u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-      const Unit un = get_unit(p, n_tiles, u);
-      if (un.rows <= 0 || un.ad.rank == 0) continue;
-      const int rcs = (un.ad.rp + KC - 1) / KC;
-      const uint32_t bytes = is_a ? un.ad.rank * 128 : kBPlane;  // of a piece
-      const uint8_t* src = is_a ? un.ad.ta : un.ad.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
+    UnitCursor uc;
+    Unit un;
+    while (ok && uc.next<false, true>(un, units, ufull, uempty, abort_flag, err)) {
+      if (un.rank == 0) continue;
+      const int rcs = (un.rp + KC - 1) / KC;
+      const uint32_t bytes = is_a ? un.rank * 128 : kBPlane;  // of a piece
+      const uint8_t* src = is_a ? un.ta : un.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
       for (int n = is_a ? k_stages * 2 * PW : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
         ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
         if (!ok) break;

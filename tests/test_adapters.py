@@ -352,6 +352,21 @@ def test_lowrank_int8_codes(ctx, codes, w):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [17, 23, 33, 64])
+@pytest.mark.parametrize("k,n,x", [(768, 256, "bf16"), (32, 40, "f32")])
+def test_lowrank_many_short_tiles(ctx, rows, k, n, x):
+    # more tiles than SMs, each its own adapter's, most of them shorter than a full one; then a few full ones
+    count = 700
+    c = LowRankCase(ctx, [rows] * count + [200], [i % 40 if i % 7 else -1 for i in range(count)] + [40],
+                    [3 + i % 30 for i in range(40)] + [8], k, n, x=x, w="f16", seed=rows)
+    c.run(ctx)
+    c.close()
+    c = LowRankCase(ctx, [rows] * 60, list(range(60)), [8 + i % 3 for i in range(60)], k, n, x=x, w="bf16", seed=rows)
+    c.run(ctx)
+    c.close()
+
+
+@pytest.mark.gpu
 def test_lowrank_empty_batch_writes_nothing(ctx):
     import torch
     c = LowRankCase(ctx, [0, 0], [0, -1], [4], 8, 8)
