@@ -5,6 +5,7 @@
 // without adapters.
 #include "adapters.h"
 
+#include <array>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -61,7 +62,7 @@ AdapterPlanDev plan_device(const sem_adapter_plan* p) {
   const int32_t* maps = p->maps.as<int32_t>();
   return AdapterPlanDev{reinterpret_cast<const int32_t*>(up), tiles,
                         tiles + adapter_plan_max_large(p->max_rows, p->max_seqs), maps, maps + p->max_rows,
-                        maps + 2 * p->max_rows};
+                        maps + 2 * p->max_rows, p->max_rows};
 }
 
 int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapters, int32_t n_seqs, cudaStream_t st) {
@@ -141,7 +142,8 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
   const int32_t ka = (int32_t)round_up(k_in, 64);
   // host image: the adapter table, then every adapter's a and b, rows padded with zeros
   size_t bytes = (size_t)round_up((int64_t)n_adapters * sizeof(LowRankAdapter), 256);
-  std::vector<size_t> at_a(n_adapters), at_b(n_adapters), at_ta(n_adapters), at_tb(n_adapters);
+  std::vector<size_t> at_a(n_adapters), at_b(n_adapters), at_tb(n_adapters), at_us(n_adapters);
+  std::vector<std::array<size_t, 3>> at_ta(n_adapters);
   int32_t max_rank = 0;
   for (int32_t i = 0; i < n_adapters; ++i) {
     const int64_t rp = round_up(ranks[i], 8);
@@ -154,10 +156,15 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
   // behind the image, filled on the device: the weights as the tensor-core kernel's tiles
   size_t total = bytes;
   for (int32_t i = 0; i < n_adapters; ++i) {
-    at_ta[i] = total;
-    total += lowrank_tile_bytes_a(ranks[i], ka, dtype);  // multiples of 128 bytes
+    const int32_t rp = (int32_t)round_up(ranks[i], 8);
+    for (int x = 0; x < 3; ++x) {
+      at_ta[i][x] = total;
+      total += lowrank_tile_bytes_a(ranks[i], ka, dtype, x);  // these are multiples of 128 bytes
+    }
     at_tb[i] = total;
-    total += lowrank_tile_bytes_b((int)round_up(ranks[i], 8), n_out, dtype);
+    total += lowrank_tile_bytes_b(rp, n_out, dtype);
+    at_us[i] = total;
+    total += (size_t)round_up(rp * 4, 128);
   }
   cudaError_t e = w->weights.ensure(total > 0 ? total : 256);
   if (e != cudaSuccess)
@@ -175,7 +182,14 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
     for (int32_t n = 0; r > 0 && n < n_out; ++n)
       std::memcpy(&img[at_b[i] + (size_t)n * rp * es], static_cast<const uint8_t*>(b[i]) + (size_t)n * r * es,
                   (size_t)r * es);
-    const LowRankAdapter ad{d + at_a[i], d + at_b[i], d + at_ta[i], d + at_tb[i], r, rp, scales[i]};
+    const LowRankAdapter ad{d + at_a[i],
+                            d + at_b[i],
+                            d + at_tb[i],
+                            {d + at_ta[i][0], d + at_ta[i][1], d + at_ta[i][2]},
+                            lowrank_has_unscale(dtype) ? reinterpret_cast<const float*>(d + at_us[i]) : nullptr,
+                            r,
+                            rp,
+                            scales[i]};
     table[i] = ad;
     std::memcpy(&img[(size_t)i * sizeof(LowRankAdapter)], &ad, sizeof ad);
   }

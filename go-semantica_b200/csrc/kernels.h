@@ -271,6 +271,7 @@ struct AdapterPlanDev {
   const int32_t* pos_row;      // [rows] the row at each position
   const int32_t* pos_seq;      // [rows] and its sequence
   const int32_t* row_adapter;  // [rows]
+  int64_t max_rows;            // the plan's capacity
 };
 // pos_row, pos_seq and row_adapter from the sorted sequences: sequence i of
 // the order holds positions [pos[i], pos[i + 1]) and rows from row0[i] on.
@@ -287,8 +288,10 @@ constexpr int kLowRankMaxRank = 128;
 struct LowRankAdapter {
   const void* a;
   const void* b;
-  const uint8_t* ta;  // a and b as the tensor-core kernel's tiles (launch_lowrank_tiles)
+  // the tensor-core kernel's tiles (launch_lowrank_tiles): b, and a for x of each DType
   const uint8_t* tb;
+  const uint8_t* ta[3];
+  const float* unscale;  // [rp] factors of ta[kDtF16]'s ranks, null: 1
   int32_t rank, rp;
   float scale;
 };
@@ -319,9 +322,11 @@ cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& 
 // receives error bits if a pipeline wait times out.
 cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
                               const LowRankArgs& args, uint32_t* err, cudaStream_t stream);
-// Bytes of an adapter's ta and tb, and the kernel that fills them from a and b.
-size_t lowrank_tile_bytes_a(int rank, int ka, int wtype);
+// Bytes of an adapter's ta[xtype] and tb, whether it has unscale factors, and
+// the kernels that fill them from a and b.
+size_t lowrank_tile_bytes_a(int rank, int ka, int wtype, int xtype);
 size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype);
+inline bool lowrank_has_unscale(int wtype) { return wtype != kDtF16; }
 cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, int ka, int wtype,
                                  cudaStream_t stream);
 

@@ -9,19 +9,23 @@
 // along the channels of a row, coalesced. Two expand accumulators hold the
 // even and the odd channels of 256: a thread owns two neighbours.
 //
-// Numbers. The operands are tf32 (11 significant bits): fp16, bf16 and INT8
-// codes are exact in it; a float32 value v goes in as two parts, hi = v cut to
-// 11 bits and lo = v - hi cut to 11 bits, and
-// hi hi + hi lo + lo hi are accumulated in float32 in TMEM, so products keep at
-// least 21 bits. t stays float32 between the products (hi and lo again). Only
+// Numbers. No operand loses bits that count: every value goes in as the parts
+// that give at least 21 bits, and the products of parts (all but those below
+// 2^-22) are accumulated in float32 in TMEM. Shrink of float32 rows: tf32 (11
+// bits), x and float32 weights as hi + lo. Shrink of 16-bit rows (and INT8
+// codes held as fp16): kind::f16 on the rows as they are, A in x's type: one
+// part where the types are the same, else two bf16 parts of fp16, three bf16
+// parts of float32, or two fp16 parts of a rank's weights scaled by a power of
+// two (undone in t). Expand: tf32, t as hi + lo, B as stored or hi + lo. Only
 // y's own rounding loses bits.
 //
 // Bound by HBM at the ranks in use: a row moves k |x| + 2 n |y| bytes and
 // needs 2 r (k + n) flops (r = 16, 768 x 768, float32: 9.2 KB against 49
 // kflop, two products each: 0.02 of the tensor pipe). So the work is to keep
 // loads in flight and every other role short:
-//   - X warps (8): rows of x (any order and alignment) by asynchronous copies
-//     to where their operand goes, 128-byte swizzled, then split in place;
+//   - X warps (8): rows of x to where their operand goes, 128-byte swizzled:
+//     by TMA where a whole unit's rows follow each other, by asynchronous
+//     copies otherwise (any order and alignment); float32 is then split there;
 //   - two copy threads: the adapter's A and B tiles, which the bank keeps as
 //     tf32 planes in the swizzled layout, with one bulk copy per plane;
 //   - a shrink and an expand MMA thread, so that the shrink of later units
@@ -40,6 +44,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "sm100.cuh"
+#include "tmap.h"
 
 namespace sem {
 
@@ -61,7 +66,7 @@ constexpr int kRt = 64;  // rows per unit at most
 static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile or a part of one");
 constexpr int kMaxSlots = 8;
 constexpr int kBPlane = 128 * 128;  // one plane of a slot of B: 128 channels x 128 bytes
-constexpr int kMiscBytes = 1280;
+constexpr int kMiscBytes = 1792;
 constexpr int kEpiRows = 8;  // rows per batch of an epilogue warp's ring of base
 constexpr int kMaxSmem = 232448;  // an MMA reads 128 rows from a slot's start: a short slot's run on into sW and sT
 
@@ -82,6 +87,11 @@ __device__ __forceinline__ bool elect_lane() {
       "selp.u32 %0, 1, 0, p;\n\t}\n"
       : "=r"(p));
   return p != 0;
+}
+// kind::f16, fp16 (0) or bf16 (1) operands.
+__host__ __device__ constexpr uint32_t idesc_16(int fmt, int M, int N) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -221,8 +231,9 @@ struct ShrinkAcc {
 // the dependent loads of tile and adapter cost no role anything) and passes it
 // on through a ring in shared memory; the last entry has no rows.
 struct alignas(16) Unit {
-  const uint8_t* ta;
+  const uint8_t* ta;     // A's tiles for this x
   const uint8_t* tb;
+  const float* unscale;  // factors of t's ranks, or null
   int32_t pos0, rows;  // positions
   int32_t row0;        // their rows follow each other from here, or -1
   int32_t c0, c1;      // chunks of 256 output channels
@@ -232,14 +243,24 @@ struct alignas(16) Unit {
 constexpr int kUnitSlots = 8;  // above the four units that an epilogue warp's copies can be ahead of its stores
 constexpr int kUnitReaders = kXWarps + kEpiWarps + kTWarps + 4;
 
+// Parts of A for x of type XT and weights of type wtype.
+__host__ __device__ constexpr int a_parts(int xtype, int wtype) {
+  return xtype == kDtF32 ? (wtype == kDtF32 ? 2 : 1) : xtype == wtype ? 1 : xtype == kDtBF16 && wtype == kDtF32 ? 3 : 2;
+}
+template <class XT>
+__host__ __device__ constexpr int dtype_of() {
+  return std::is_same<XT, float>::value ? kDtF32 : std::is_same<XT, __half>::value ? kDtF16 : kDtBF16;
+}
+
 struct TcParams {
+  CUtensorMap tm_x, tm_b;  // rows of x (boxes of rt rows x 128 bytes, swizzled) and of base (8 rows x 64 channels)
   LowRankBank bank;
   AdapterPlanDev plan;
   LowRankArgs a;
   int32_t rt, splits;        // rows per unit (16, 32 or 64), shares of the output channels
   int32_t x_slots, a_slots, b_slots, t_bufs;  // ring depths
   int32_t epi_ring;  // bytes of an epilogue warp's ring: 2048 or 4096
-  int32_t x_vec;   // rows of x start on 16 bytes
+  int32_t x_vec;   // rows of x start on 16 bytes (16-byte copies, TMA)
   int32_t b_copy;  // bytes of a copy that base's rows are aligned for: 16, 4 or 2 (none, element loads)
   int32_t y_pair;  // y's channels can be stored in pairs
   uint32_t* err;
@@ -247,6 +268,7 @@ struct TcParams {
 
 // Unit u. Sub-tiles of the same number lie together, so that those behind a
 // tile's last row come last.
+template <int XTYPE>
 __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t u) {
   Unit r;
   const int split = (int)(u % p.splits);
@@ -260,11 +282,13 @@ __device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t
   r.c0 = chunks * split / p.splits;
   r.c1 = chunks * (split + 1) / p.splits;
   r.ta = r.tb = nullptr;
+  r.unscale = nullptr;
   r.rank = r.rp = 0;
   r.scale = 0.0f;
   if (r.rows > 0 && tl.adapter >= 0 && tl.adapter < p.bank.n_adapters) {
     const LowRankAdapter ad = p.bank.adapters[tl.adapter];
-    r.ta = ad.ta, r.tb = ad.tb, r.rank = ad.rank, r.rp = ad.rp, r.scale = ad.scale;
+    r.ta = ad.ta[XTYPE], r.tb = ad.tb, r.rank = ad.rank, r.rp = ad.rp, r.scale = ad.scale;
+    if (XTYPE == kDtF16) r.unscale = ad.unscale;
   }
   return r;
 }
@@ -292,16 +316,19 @@ struct UnitCursor {
 
 template <class XT, class YT>
 __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_constant__ TcParams p) {
-  constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;  // planes of x
+  constexpr int XTYPE = dtype_of<XT>();
+  constexpr int PX = XTYPE == kDtF32 ? 2 : 1;                 // planes of x
+  constexpr int XA = XTYPE == kDtF32 ? 2 : 1;                 // 128-byte rows of a plane per stage
   constexpr int XE = 16 / sizeof(XT);                         // elements of a 16-byte copy
   constexpr int XL = KS / XE;                                 // copies per row and stage
   constexpr int XR = kXWarps * 32 / XL;                       // rows per pass of the X warps
   constexpr int XV = kRt / XR;                                // passes
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  const int PW = p.bank.wtype == kDtF32 ? 2 : 1;  // planes of the weights
-  const int x_atom = p.rt * 128, x_slot = PX * 2 * x_atom;  // [plane][32 channels][rt rows][128 B]
-  const int a_slot = ((p.bank.max_rank + 15) & ~15) * 128;  // a piece of A: the ranks of 32 channels of a plane
+  const int PW = p.bank.wtype == kDtF32 ? 2 : 1;  // planes of B
+  const int PA = a_parts(XTYPE, p.bank.wtype);    // parts of A
+  const int x_atom = p.rt * 128, x_slot = PX * XA * x_atom;  // [plane][128 bytes of channels][rt rows][128 B]
+  const int a_slot = ((p.bank.max_rank + 15) & ~15) * 128;  // a piece of A: the ranks' 128-byte rows
   const int t_plane = p.rt * 128, t_chunks = (p.bank.max_rank + KC - 1) / KC;  // [chunk][hi, lo][rt rows][128 B]
   uint8_t* sX = smem;
   uint8_t* sA = sX + p.x_slots * x_slot;
@@ -325,10 +352,13 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   uint64_t* drain = dempty + 2;           // [2] the MMA threads' last MMAs
   uint64_t* ufull = drain + 2;            // the ring of units
   uint64_t* uempty = ufull + kUnitSlots;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(uempty + kUnitSlots);
+  uint64_t* xraw = uempty + kUnitSlots;    // float32 rows have arrived
+  uint64_t* efull = xraw + kMaxSlots;      // [epilogue warp][4] a batch of base has arrived
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(efull + kEpiWarps * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
-  Unit* units = reinterpret_cast<Unit*>(misc + 768);
-  static_assert((6 * kMaxSlots + 14 + 2 * kUnitSlots) * 8 + 8 <= 768 && 768 + sizeof(Unit) * kUnitSlots <= kMiscBytes, "");
+  Unit* units = reinterpret_cast<Unit*>(misc + 1280);
+  static_assert((7 * kMaxSlots + 14 + 2 * kUnitSlots + kEpiWarps * 4) * 8 + 8 <= 1280 &&
+                    1280 + sizeof(Unit) * kUnitSlots <= kMiscBytes, "barriers and units");
   uint32_t* err = p.err ? p.err : &g_lowrank_error;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -340,7 +370,9 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       mbar_init(&aempty[i], 1);
       mbar_init(&bfull[i], 1);
       mbar_init(&bempty[i], 1);
+      mbar_init(&xraw[i], 1);
     }
+    for (int i = 0; i < kEpiWarps * 4; ++i) mbar_init(&efull[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tafull[i], 1);
       mbar_init(&taempty[i], kTWarps);
@@ -365,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   const int k_stages = p.bank.ka / KS;
 
   if (warp < kXWarps) {
-    // ---------------- x: global -> swizzled shared memory, split in place ----------------
+    // ---------------- x: global -> swizzled shared memory; float32 split in place ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsX));
     const int k = p.bank.k_in;
     const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
@@ -373,12 +405,13 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     const XT* row[XV];
     // the cursor of the copies: a unit, its stage ks
     UnitCursor uc;
-    int ks = 0, passes = 0;
+    int ks = 0, passes = 0, tma_row = -1;
     auto open = [&]() -> bool {  // the next unit with something to add
       Unit un;
       do {
         if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) return false;
       } while (un.rank == 0);
+      tma_row = p.x_vec && un.rows == p.rt ? un.row0 : -1;  // a box holds rows of the unit only
       passes = (un.rows + XR - 1) / XR;  // later ones have no rows
 #pragma unroll
       for (int i = 0; i < XV; ++i) {  // behind the last row: that row again
@@ -389,42 +422,57 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       ks = 0;
       return true;
     };
-    // This thread's 16-byte pieces of its first row in a slot (its other rows are multiples of 8 further). A copy
-    // of 16-bit values lands where the first or, in lanes of the upper 32 channels, the second of its two pieces
-    // goes, and that piece is written first: the lanes of a row then touch different banks.
+    // this thread's 16-byte piece of its first row in a slot (its other rows are multiples of 8 further)
     static_assert(XR % 8 == 0, "swizzle");
-    const bool upper = PX == 1 && col >= KC;
-    const uint32_t at0 = (col / KC) * x_atom + r0 * 128 + (((col % KC) / 4) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
-    const uint32_t land = upper ? at1 : at0;
+    constexpr int XC = 128 / sizeof(XT);  // channels of a 128-byte row
+    const uint32_t at0 = (col / XC) * x_atom + r0 * 128 + ((col % XC / XE) ^ (r0 & 7)) * 16;
     Ring ir, xr;  // copies issued, stages done
+    uint32_t by_tma = 0;  // slots on their way by TMA
     bool ok = true, more = open();
     int pending = 0;
-    auto issue = [&]() {  // the cursor's stage, one group (an empty one at the end)
+    auto issue = [&]() {  // the cursor's stage, with one group of copies (an empty one by TMA, and at the end)
       if (more) {
         ok = warp_wait(&xempty[ir.slot], ir.parity ^ 1, abort_flag, err, 1u);
         if (!ok) return;
-        uint8_t* dst = sX + ir.slot * x_slot + land;
-        const int c = ks * KS + col;
+        uint8_t* dst = sX + ir.slot * x_slot;
+        by_tma &= ~(1u << ir.slot);
+        if (tma_row >= 0) {
+          by_tma |= 1u << ir.slot;
+          // float32: the X warps take over when the bytes are there; 16-bit: they go straight to the MMAs
+          uint64_t* bar = PX == 2 ? &xraw[ir.slot] : &xfull[ir.slot];
+          if (lane == 0) {
+            if (warp == 0) {
+              mbar_arrive_expect_tx(bar, XA * x_atom);
 #pragma unroll
-        for (int i = 0; i < XV; ++i) {
-          if (i >= passes || r0 + i * XR >= p.rt) break;
-          if (ks < full_stages) {
-            copy16(smem_u32(dst) + i * XR * 128, row[i] + ks * KS, 16);
-          } else {
-            XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
-#pragma unroll
-            for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1) - col];
-            uint32_t v[4];
-            if constexpr (PX == 2) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] = c + j < k ? __float_as_uint(e[j]) : 0u;
-            } else {
-              const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                v[j] = (c + 2 * j < k ? h[2 * j] : 0u) | (c + 2 * j + 1 < k ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+              for (int i = 0; i < XA; ++i) tma_load_2d(&p.tm_x, bar, dst + i * x_atom, ks * KS + i * XC, tma_row);
+            } else if (PX == 1) {
+              mbar_arrive(bar);
             }
-            *reinterpret_cast<uint4*>(dst + i * XR * 128) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        } else {
+          if (PX == 2 && warp == 0 && lane == 0) mbar_arrive(&xraw[ir.slot]);  // its phases count stages
+          const int c = ks * KS + col;
+#pragma unroll
+          for (int i = 0; i < XV; ++i) {
+            if (i >= passes || r0 + i * XR >= p.rt) break;
+            if (ks < full_stages) {
+              copy16(smem_u32(dst) + at0 + i * XR * 128, row[i] + ks * KS, 16);
+            } else {
+              XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
+#pragma unroll
+              for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1) - col];
+              uint32_t v[4];
+              if constexpr (PX == 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = c + j < k ? __float_as_uint(e[j]) : 0u;
+              } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  v[j] = (c + 2 * j < k ? h[2 * j] : 0u) | (c + 2 * j + 1 < k ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+              }
+              *reinterpret_cast<uint4*>(dst + at0 + i * XR * 128) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
           }
         }
         ir.next(p.x_slots);
@@ -436,43 +484,37 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     const int depth = p.x_slots - 1;
     for (int d = 0; ok && d < depth; ++d) issue();
     while (ok && pending > 0) {
-      copy_wait(depth - 1);  // the oldest stage of this thread has landed
-      uint8_t* dst = sX + xr.slot * x_slot;
+      copy_wait(depth - 1);  // the oldest stage of this thread's own copies has landed
+      if (PX == 2) {
+        ok = warp_wait(&xraw[xr.slot], xr.parity, abort_flag, err, 16384u);
+        if (!ok) break;
+        uint8_t* dst = sX + xr.slot * x_slot + at0;
 #pragma unroll
-      for (int i = 0; i < XV; ++i) {
-        if (r0 + i * XR >= p.rt) break;
-        const uint4 v = *reinterpret_cast<const uint4*>(dst + land + i * XR * 128);
-        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-        if constexpr (PX == 2) {
-          float hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(e[j]), hi[j], lo[j]);
-          *reinterpret_cast<float4*>(dst + at0 + i * XR * 128) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<float4*>(dst + 2 * x_atom + at0 + i * XR * 128) = make_float4(lo[0], lo[1], lo[2], lo[3]);
-        } else {
-          float f[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (std::is_same<XT, __half>::value) {
-              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
-              f[2 * j] = g.x, f[2 * j + 1] = g.y;
-            } else {
-              f[2 * j] = __uint_as_float(e[j] << 16), f[2 * j + 1] = __uint_as_float(e[j] & 0xffff0000u);
-            }
-          }
-          const float4 p0 = make_float4(f[0], f[1], f[2], f[3]), p1 = make_float4(f[4], f[5], f[6], f[7]);
-          *reinterpret_cast<float4*>(dst + land + i * XR * 128) = upper ? p1 : p0;
-          *reinterpret_cast<float4*>(dst + (land ^ 16) + i * XR * 128) = upper ? p0 : p1;
+        for (int i = 0; i < XV; ++i) {
+          if (r0 + i * XR >= p.rt) break;
+          const float4 v = *reinterpret_cast<const float4*>(dst + i * XR * 128);
+          float4 hi, lo;
+          split_tf32(v.x, hi.x, lo.x);
+          split_tf32(v.y, hi.y, lo.y);
+          split_tf32(v.z, hi.z, lo.z);
+          split_tf32(v.w, hi.w, lo.w);
+          *reinterpret_cast<float4*>(dst + i * XR * 128) = hi;
+          *reinterpret_cast<float4*>(dst + XA * x_atom + i * XR * 128) = lo;
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&xfull[xr.slot]);
+      if (PX == 2 || !(by_tma >> xr.slot & 1)) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xfull[xr.slot]);
+      }
       xr.next(p.x_slots);
       --pending;
       issue();
     }
     cp_async_wait<0>();
+    // given up: loads in flight land before the CTA's shared memory is released
+    for (; !ok && pending > 0; --pending, xr.next(p.x_slots))
+      mbar_wait_drain(PX == 2 ? &xraw[xr.slot] : &xfull[xr.slot], xr.parity);
   } else if (warp < kWarpT) {
     // ---------------- epilogue: base + accumulators -> y ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
@@ -489,7 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     // (that of row i0), or lane i holds row i0 + i.
     UnitCursor fu, uc;
     int fc = 0, fc1 = 0, fi = 0, fi1 = 0, frow0 = 0, frow = 0;
-    uint32_t fslot = ring;
+    uint64_t* bars = efull + (warp - kWarpEpi) * 4;
+    Ring fr, er;      // batches copied, batches used
     int ahead = 0;    // units that fu is ahead of uc: the ring holds kUnitSlots, and uc alone frees them
     int filled = 0;   // batches copied and not yet used
     bool more = false, end = base == nullptr;
@@ -519,19 +562,24 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           return frow0 >= 0 ? (int64_t)frow0 + min(fi + r, fi1 - 1) - i0
                             : (int64_t)__shfl_sync(0xffffffffu, frow, fi - i0 + r);
         };
-        if (p.b_copy == 16) {
+        const uint32_t fslot = ring + fr.slot * (B * RB);
+        const bool tma = p.b_copy == 16 && frow0 >= 0 && fi + B <= fi1;  // a box holds rows of the unit only
+        if (lane == 0) {
+          if (tma) {
+            mbar_arrive_expect_tx(&bars[fr.slot], B * RB);
+            tma_load_2d(&p.tm_b, &bars[fr.slot], sE + (fslot - smem_u32(sE)), ch, frow0 + fi - i0);
+          } else {
+            mbar_arrive(&bars[fr.slot]);  // its phases count batches
+          }
+        }
+        if (tma) {
+        } else if (p.b_copy == 16) {
           constexpr int LPR = RB / 16, E16 = 16 / sizeof(YT), RPI = 32 / LPR;  // lanes per row, rows per instruction
           const int c = lane % LPR * E16, bytes = max(0, min(16, (in - c) * (int)sizeof(YT)));
           const uint32_t dst = fslot + lane / LPR * RB + c * sizeof(YT);
           const YT* col = base + (bytes ? ch + c : 0);
-          if (frow0 >= 0 && fi + B <= fi1) {
-            const YT* src = col + (int64_t)(frow0 + fi - i0 + lane / LPR) * p.a.ldb;
 #pragma unroll
-            for (int j = 0; j < B; j += RPI, src += RPI * p.a.ldb) copy16(dst + j * RB, src, bytes);
-          } else {
-#pragma unroll
-            for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + row_of(j + lane / LPR) * p.a.ldb, bytes);
-          }
+          for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + row_of(j + lane / LPR) * p.a.ldb, bytes);
         } else if (p.b_copy == 4) {
           constexpr int E4 = 4 / sizeof(YT);
 #pragma unroll 2
@@ -556,8 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 #pragma unroll
           for (int r = 0; r < B; ++r) dst[r * 64 + lane] = v0[r], dst[r * 64 + lane + 32] = v1[r];
         }
-        fslot += B * RB;
-        if (fslot == ring + p.epi_ring) fslot = ring;
+        fr.next(nb);
         fi += B;
         if (fi >= fi1) {
           fi = i0;
@@ -568,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       }
     };
     for (int b = 0; b < nb; ++b) fill();
-    uint32_t d = 0, slot = ring;
+    uint32_t d = 0;
     bool ok = true;
     Unit un;
     while (ok) {
@@ -597,13 +644,15 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           Pair b[B];
           if (base) {
             if (!filled) fill();  // the cursor was at its limit
-            copy_wait(--filled);
-            __syncwarp();
-            const uint8_t* src = sE + (slot - smem_u32(sE)) + lane * 2 * sizeof(YT);
+            copy_wait(filled - 1);
+            ok = warp_wait(&bars[er.slot], er.parity, abort_flag, err, 32768u);
+            if (!ok) break;
+            __syncwarp();  // the other lanes' copies
+            const uint8_t* src = sE + (ring - smem_u32(sE)) + er.slot * (B * RB) + lane * 2 * sizeof(YT);
 #pragma unroll
             for (int j = 0; j < B; ++j) b[j] = *reinterpret_cast<const Pair*>(src + j * RB);
-            slot += B * RB;
-            if (slot == ring + p.epi_ring) slot = ring;
+            er.next(nb);
+            --filled;
             __syncwarp();
             fill();
           } else {
@@ -642,12 +691,14 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             }
           }
         }
+        if (!ok) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&dempty[d & 1]);
       }
     }
     cp_async_wait<0>();
+    for (; !ok && filled > 0; --filled, er.next(nb)) mbar_wait_drain(&bars[er.slot], er.parity);  // as above
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp < kWarpShrink) {
@@ -664,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       if (p.a.absmax && row < un.rows)
         sc = __fmul_rn(sc, __fdiv_rn(__uint_as_float(p.a.absmax[p.a.per_seq ? p.plan.pos_seq[un.pos0 + row] : 0]),
                                      127.0f));
-      const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PW == 2, k_stages);
+      const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PA > 1, k_stages);
       ok = warp_wait(&tafull[(q & (sa.bufs - 1))], (q >> (sa.bufs - 1)) & 1, abort_flag, err, 4u) &&
            warp_wait(&tfree[tr.slot], tr.parity ^ 1, abort_flag, err, 8u);
       if (!ok) break;
@@ -688,6 +739,10 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             reg_barrier8(v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = __fadd_rn(t[e], __uint_as_float(v[e]));
+          }
+          if (XTYPE == kDtF16 && un.unscale) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], __ldg(un.unscale + j + e));
           }
           float hi[8], lo[8];
 #pragma unroll
@@ -722,8 +777,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       Unit un;
       while (ok && uc.next<false, true>(un, units, ufull, uempty, abort_flag, err)) {
         if (un.rank == 0) continue;
-        const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PW == 2, k_stages);
-        const uint32_t set = q & (sa.bufs - 1), id = idesc_tf32(128, sa.width);
+        const ShrinkAcc sa(p.bank.max_rank, un.rank, PX == 2 || PA > 1, k_stages);
+        const uint32_t set = q & (sa.bufs - 1), id = XTYPE == kDtF32 ? idesc_tf32(128, sa.width) : idesc_16(XTYPE == kDtBF16, 128, sa.width);
         ok = stage_wait(&taempty[set], ((q >> (sa.bufs - 1)) & 1) ^ 1, abort_flag, err, 16u);
         tc_fence_after();
         const uint32_t acc0 = tmem + set * 128u, acc_lo = acc0 + (uint32_t)(sa.hi_parts * sa.width);
@@ -735,8 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u);
             tc_fence_after();
             const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot);
-            // a piece of A (32 channels of a plane) against the planes of x
-            auto piece = [&](int at, bool low) {
+            // a piece of A against x: `at` its 128-byte rows, `low` all but its first part
+            auto piece = [&](int at, bool low, bool first) {
               if (!ok) return;
               ok = stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
               if (!ok) return;
@@ -744,25 +799,32 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
               const uint32_t x = x0 + at * (x_atom >> 4), w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
               if (!low) {
 #pragma unroll
-                for (int s = 0; s < KC / 8; ++s) {
-                  umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, s > 0 || at > 0 ? 1 : more);
-                  if (PX == 2)
+                for (int s = 0; s < 4; ++s) {
+                  const uint32_t on = s > 0 || at > 0 ? 1 : more;
+                  if (PX == 2) {
+                    umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, on);
                     umma_tf32(acc_lo, desc_at(x + (x_atom >> 3) + 2 * s), desc_at(w + 2 * s), id,
                               s > 0 || at > 0 ? 1 : c > 0);
+                  } else {
+                    umma_f16(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, on);
+                  }
                 }
               } else {
 #pragma unroll
-                for (int s = 0; s < KC / 8; ++s)
-                  umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, PX == 2 || s > 0 || at > 0 ? 1 : c > 0);
+                for (int s = 0; s < 4; ++s) {
+                  if (PX == 2) umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, 1);
+                  else umma_f16(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, s > 0 || !first ? 1 : c > 0);
+                }
               }
               umma_commit(&aempty[ar.slot]);
               ar.next(p.a_slots);
             };
-            piece(0, false);
-            piece(1, false);
-            if (PW == 2) {
-              piece(0, true);
-              piece(1, true);
+            piece(0, false, true);
+            if (PX == 2) piece(1, false, true);
+            if (PA > 1) {
+              piece(0, true, true);
+              if (PX == 2) piece(1, true, true);
+              if (PX == 1 && PA > 2) piece(0, true, false);
             }
             more = 1;
             if (!ok) break;
@@ -836,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int64_t u = first + lane * (int64_t)gridDim.x;
       Unit un;
       un.rows = 0;
-      if (u < n_units) un = get_unit(p, n_tiles, u);
+      if (u < n_units) un = get_unit<XTYPE>(p, n_tiles, u);
       uint32_t todo = __ballot_sync(0xffffffffu, un.rows > 0 && un.c1 > un.c0 && (un.rank > 0 || !in_place));
       const bool last = first + 32 * (int64_t)gridDim.x >= n_units;
       while (ok && (todo || last)) {
@@ -871,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int rcs = (un.rp + KC - 1) / KC;
       const uint32_t bytes = is_a ? un.rank * 128 : kBPlane;  // of a piece
       const uint8_t* src = is_a ? un.ta : un.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
-      for (int n = is_a ? k_stages * 2 * PW : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
+      for (int n = is_a ? k_stages * XA * PA : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
         ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
         if (!ok) break;
         mbar_arrive_expect_tx(&full[r.slot], bytes);
@@ -912,7 +974,7 @@ __global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int
       c = kk % KC;
       const int64_t atom = (int64_t)ad.rank * 128;
       plane = 2 * atom;
-      tile = const_cast<uint8_t*>(ad.ta) + (int64_t)(kk / KS) * planes * plane + kk % KS / KC * atom;
+      tile = const_cast<uint8_t*>(ad.ta[kDtF32]) + (int64_t)(kk / KS) * planes * plane + kk % KS / KC * atom;
       if (kk < k_in) v = as_f32(static_cast<const WT*>(ad.a)[i]);
     } else {
       const int64_t b = i - na, t = b / (128 * KC);
@@ -936,9 +998,50 @@ __global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int
   }
 }
 
+// A's tiles for 16-bit x: [k stage][part][rank rows of 64 channels], swizzled
+// the same way. A CTA per rank. fp16 parts of other types: the rank's weights
+// times the power of two that brings the largest to [2^13, 2^14).
+template <class WT>
+__global__ void lowrank_tiles16_kernel(LowRankAdapter ad, int k_in, int ka, int parts_f16, int parts_bf16) {
+  __shared__ float s_max[8];
+  const int j = blockIdx.x;
+  const WT* w = static_cast<const WT*>(ad.a) + (int64_t)j * ka;
+  float top = 0.0f;
+  for (int k = threadIdx.x; k < k_in; k += blockDim.x) top = fmaxf(top, fabsf(as_f32(w[k])));
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
+  __syncthreads();
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) top = fmaxf(top, s_max[i]);
+  int up = 0;
+  if (ad.unscale && top > 0.0f && top < __uint_as_float(0x7f800000u)) up = min(13 - ilogbf(top), 100);
+  if (ad.unscale && threadIdx.x == 0) const_cast<float*>(ad.unscale)[j] = ldexpf(1.0f, -up);
+  auto put = [&](int xtype, int parts, int part, int k, uint16_t bits) {
+    uint8_t* row = const_cast<uint8_t*>(ad.ta[xtype]) + ((int64_t)(k / KS * parts + part) * ad.rank + j) * 128;
+    const int c = k % KS;
+    *reinterpret_cast<uint16_t*>(row + (((c >> 3) ^ (j & 7)) * 16) + (c & 7) * 2) = bits;
+  };
+  for (int k = threadIdx.x; k < ka; k += blockDim.x) {
+    const float v = k < k_in ? as_f32(w[k]) : 0.0f;
+    const float f = ldexpf(v, up);
+    const __half h = __float2half_rn(f);
+    put(kDtF16, parts_f16, 0, k, __half_as_ushort(h));
+    if (parts_f16 > 1) {
+      const float rest = __fsub_rn(f, __half2float(h));
+      put(kDtF16, parts_f16, 1, k, __half_as_ushort(__float2half_rn(isfinite(rest) ? rest : 0.0f)));
+    }
+    float rest = v;
+    for (int part = 0; part < parts_bf16; ++part) {  // cut, not rounded: no part overflows
+      const uint32_t bits = __float_as_uint(rest) & 0xffff0000u;
+      put(kDtBF16, parts_bf16, part, k, (uint16_t)(bits >> 16));
+      const float less = __fsub_rn(rest, __uint_as_float(bits));
+      rest = isfinite(less) ? less : 0.0f;
+    }
+  }
+}
+
 template <class XT, class YT>
 cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
-  constexpr int PX = std::is_same<XT, float>::value ? 2 : 1;
+  constexpr int XTYPE = dtype_of<XT>(), PX = XTYPE == kDtF32 ? 2 : 1, XA = PX;
   const int chunks = (p.bank.n_out + 255) / 256;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -952,7 +1055,7 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = (p.bank.max_rank + 15) / 16 * 16 * 128;
   int smem = 0;
   for (; p.rt >= 16; p.rt /= 2) {
-    const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * 2 * p.rt * 128;
+    const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * XA * p.rt * 128;
     int left = kMaxSmem - 1024 - kMiscBytes - kEpiWarps * 2048 - 2 * (kBPlane + a_slot + x_slot) - t_buf;
     if (left < 0) continue;
     p.t_bufs = 1, p.a_slots = p.b_slots = p.x_slots = 2, p.epi_ring = 2048;
@@ -979,6 +1082,21 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
              : (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 4 == 0 ? 4 : 2;
   p.y_pair = p.bank.n_out % 2 == 0 &&
              (reinterpret_cast<uintptr_t>(p.a.y) | (uint64_t)(p.a.ldy * sizeof(YT))) % (2 * sizeof(YT)) == 0;
+  // maps over as many rows as a plan can have; a box is loaded only where a unit has all its rows
+  auto map = [&](CUtensorMap* m, const void* at, int type, int64_t cols, int64_t ld, uint32_t bc, uint32_t br,
+                 CUtensorMapSwizzle swz) {
+    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)(p.plan.max_rows > 0 ? p.plan.max_rows : 1)};
+    const uint64_t strides[1] = {(uint64_t)ld * (type == kDtF32 ? 4 : 2)};
+    const uint32_t box[2] = {bc, br};
+    return tmap_nd(m, type == kDtF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                      : type == kDtF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   at, 2, dims, strides, box, swz);
+  };
+  if (p.x_vec)
+    e = map(&p.tm_x, p.a.x, XTYPE, p.bank.k_in, p.a.ldx, 128 / sizeof(XT), p.rt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (e == cudaSuccess && base && p.b_copy == 16)
+    e = map(&p.tm_b, p.a.base, dtype_of<YT>(), p.bank.n_out, p.a.ldb, 64, kEpiRows, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(lowrank_tc_kernel<XT, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
@@ -988,8 +1106,8 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
 
 }  // namespace
 
-size_t lowrank_tile_bytes_a(int rank, int ka, int wtype) {
-  return (size_t)(ka / KC) * rank * 128 * (wtype == kDtF32 ? 2 : 1);
+size_t lowrank_tile_bytes_a(int rank, int ka, int wtype, int xtype) {
+  return (size_t)(ka / (xtype == kDtF32 ? KC : KS)) * rank * 128 * a_parts(xtype, wtype);
 }
 size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype) {
   return (size_t)((n_out + 255) / 256 * 2) * ((rp + KC - 1) / KC) * kBPlane * (wtype == kDtF32 ? 2 : 1);
@@ -1000,9 +1118,17 @@ cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, 
   const int planes = wtype == kDtF32 ? 2 : 1;
   const int64_t n = (int64_t)ad.rank * ka + (int64_t)((n_out + 255) / 256 * 2) * ((ad.rp + KC - 1) / KC) * 128 * KC;
   const unsigned grid = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
-  if (wtype == kDtF32) lowrank_tiles_kernel<float><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
-  else if (wtype == kDtF16) lowrank_tiles_kernel<__half><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
-  else lowrank_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+  const int f16 = a_parts(kDtF16, wtype), bf16 = a_parts(kDtBF16, wtype);
+  if (wtype == kDtF32) {
+    lowrank_tiles_kernel<float><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+    lowrank_tiles16_kernel<float><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
+  } else if (wtype == kDtF16) {
+    lowrank_tiles_kernel<__half><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+    lowrank_tiles16_kernel<__half><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
+  } else {
+    lowrank_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
+    lowrank_tiles16_kernel<__nv_bfloat16><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
+  }
   return cudaGetLastError();
 }
 
