@@ -50,7 +50,7 @@ namespace sem {
 
 namespace {
 
-constexpr int kXWarps = 8, kEpiWarps = 16, kTWarps = 2;
+constexpr int kXWarps = 8, kXGroups = 2, kEpiWarps = 16, kTWarps = 2;
 constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
 constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1, kWarpUnits = kWarpB + 1;
 constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA, copy and unit warps, one idle
@@ -61,7 +61,6 @@ constexpr int kRegsX = 72, kRegsEpi = 72, kRegsRest = 40;
 static_assert(kThreads == 1024 && kXWarps * kRegsX + kEpiWarps * kRegsEpi + 8 * kRegsRest <= 32 * 64, "register split");
 static_assert(kWarpEpi % 4 == 0 && kWarpT % 4 == 0, "TMEM lane quarters go by warp index");
 constexpr int KC = 32;   // tf32 per swizzled 128-byte row
-constexpr int KS = 64;   // input channels per stage: two such rows
 constexpr int kRt = 64;  // rows per unit at most
 static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile or a part of one");
 constexpr int kMaxSlots = 8;
@@ -318,16 +317,16 @@ template <class XT, class YT>
 __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_constant__ TcParams p) {
   constexpr int XTYPE = dtype_of<XT>();
   constexpr int PX = XTYPE == kDtF32 ? 2 : 1;                 // planes of x
-  constexpr int XA = XTYPE == kDtF32 ? 2 : 1;                 // 128-byte rows of a plane per stage
+  constexpr int KS = 128 / sizeof(XT);                        // input channels per stage: a 128-byte row of x
   constexpr int XE = 16 / sizeof(XT);                         // elements of a 16-byte copy
-  constexpr int XL = KS / XE;                                 // copies per row and stage
-  constexpr int XR = kXWarps * 32 / XL;                       // rows per pass of the X warps
+  constexpr int XL = KS / XE;                                 // copies per row
+  constexpr int XR = kXWarps / kXGroups * 32 / XL;            // rows per pass of a group of X warps
   constexpr int XV = kRt / XR;                                // passes
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int PW = p.bank.wtype == kDtF32 ? 2 : 1;  // planes of B
   const int PA = a_parts(XTYPE, p.bank.wtype);    // parts of A
-  const int x_atom = p.rt * 128, x_slot = PX * XA * x_atom;  // [plane][128 bytes of channels][rt rows][128 B]
+  const int x_atom = p.rt * 128, x_slot = PX * x_atom;  // [plane][rt rows][128 B]
   const int a_slot = ((p.bank.max_rank + 15) & ~15) * 128;  // a piece of A: the ranks' 128-byte rows
   const int t_plane = p.rt * 128, t_chunks = (p.bank.max_rank + KC - 1) / KC;  // [chunk][hi, lo][rt rows][128 B]
   uint8_t* sX = smem;
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kMaxSlots; ++i) {
-      mbar_init(&xfull[i], kXWarps);
+      mbar_init(&xfull[i], kXWarps / kXGroups);
       mbar_init(&xempty[i], 1);
       mbar_init(&afull[i], 1);
       mbar_init(&aempty[i], 1);
@@ -400,33 +399,41 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     // ---------------- x: global -> swizzled shared memory; float32 split in place ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsX));
     const int k = p.bank.k_in;
-    const int tx = threadIdx.x, col = tx % XL * XE, r0 = tx / XL;
+    // The two groups of warps take the stages in turn (counted over all units), so that one converts while the other
+    // waits, fences and issues.
+    const int group = warp / (kXWarps / kXGroups), first_warp = group * (kXWarps / kXGroups);
+    const int tx = threadIdx.x - first_warp * 32, col = tx % XL * XE, r0 = tx / XL;
     const int full_stages = p.x_vec ? k / KS : 0;  // stages that 16-byte copies can take
     const XT* row[XV];
     // the cursor of the copies: a unit, its stage ks
     UnitCursor uc;
-    int ks = 0, passes = 0, tma_row = -1;
-    auto open = [&]() -> bool {  // the next unit with something to add
+    int ks = group, passes = 0, tma_row = -1;
+    auto open = [&]() -> bool {  // the unit of stage ks, which counts from the present unit's first
       Unit un;
-      do {
-        if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) return false;
-      } while (un.rank == 0);
+      for (bool have = passes > 0; !have || ks >= k_stages; have = true) {
+        if (have) ks -= k_stages;
+        do {
+          if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) return false;
+        } while (un.rank == 0);
+        passes = (un.rows + XR - 1) / XR;  // later ones have no rows
+      }
       tma_row = p.x_vec && un.rows == p.rt ? un.row0 : -1;  // a box holds rows of the unit only
-      passes = (un.rows + XR - 1) / XR;  // later ones have no rows
 #pragma unroll
       for (int i = 0; i < XV; ++i) {  // behind the last row: that row again
         const int r = min(r0 + i * XR, un.rows - 1);
         row[i] = static_cast<const XT*>(p.a.x) +
                  (int64_t)(un.row0 >= 0 ? un.row0 + r : p.plan.pos_row[un.pos0 + r]) * p.a.ldx + col;
       }
-      ks = 0;
       return true;
     };
     // this thread's 16-byte piece of its first row in a slot (its other rows are multiples of 8 further)
     static_assert(XR % 8 == 0, "swizzle");
-    constexpr int XC = 128 / sizeof(XT);  // channels of a 128-byte row
-    const uint32_t at0 = (col / XC) * x_atom + r0 * 128 + ((col % XC / XE) ^ (r0 & 7)) * 16;
+    const uint32_t at0 = r0 * 128 + ((col / XE) ^ (r0 & 7)) * 16;
+    auto step = [&](Ring& r) {  // to this group's next stage
+      for (int i = 0; i < kXGroups; ++i) r.next(p.x_slots);
+    };
     Ring ir, xr;  // copies issued, stages done
+    for (int i = 0; i < group; ++i) ir.next(p.x_slots), xr.next(p.x_slots);
     uint32_t by_tma = 0;  // slots on their way by TMA
     bool ok = true, more = open();
     int pending = 0;
@@ -441,16 +448,15 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           // float32: the X warps take over when the bytes are there; 16-bit: they go straight to the MMAs
           uint64_t* bar = PX == 2 ? &xraw[ir.slot] : &xfull[ir.slot];
           if (lane == 0) {
-            if (warp == 0) {
-              mbar_arrive_expect_tx(bar, XA * x_atom);
-#pragma unroll
-              for (int i = 0; i < XA; ++i) tma_load_2d(&p.tm_x, bar, dst + i * x_atom, ks * KS + i * XC, tma_row);
+            if (warp == first_warp) {
+              mbar_arrive_expect_tx(bar, x_atom);
+              tma_load_2d(&p.tm_x, bar, dst, ks * KS, tma_row);
             } else if (PX == 1) {
               mbar_arrive(bar);
             }
           }
         } else {
-          if (PX == 2 && warp == 0 && lane == 0) mbar_arrive(&xraw[ir.slot]);  // its phases count stages
+          if (PX == 2 && warp == first_warp && lane == 0) mbar_arrive(&xraw[ir.slot]);  // its phases count stages
           const int c = ks * KS + col;
 #pragma unroll
           for (int i = 0; i < XV; ++i) {
@@ -475,13 +481,14 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             }
           }
         }
-        ir.next(p.x_slots);
+        step(ir);
         ++pending;
-        if (++ks == k_stages) more = open();
+        ks += kXGroups;
+        if (ks >= k_stages) more = open();
       }
       cp_async_commit();
     };
-    const int depth = p.x_slots - 1;
+    const int depth = max(1, p.x_slots / kXGroups - (PX == 2 ? 1 : 0));
     for (int d = 0; ok && d < depth; ++d) issue();
     while (ok && pending > 0) {
       copy_wait(depth - 1);  // the oldest stage of this thread's own copies has landed
@@ -489,17 +496,20 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         ok = warp_wait(&xraw[xr.slot], xr.parity, abort_flag, err, 16384u);
         if (!ok) break;
         uint8_t* dst = sX + xr.slot * x_slot + at0;
+        float4 v[XV];
+#pragma unroll
+        for (int i = 0; i < XV; ++i)
+          if (r0 + i * XR < p.rt) v[i] = *reinterpret_cast<const float4*>(dst + i * XR * 128);
 #pragma unroll
         for (int i = 0; i < XV; ++i) {
           if (r0 + i * XR >= p.rt) break;
-          const float4 v = *reinterpret_cast<const float4*>(dst + i * XR * 128);
           float4 hi, lo;
-          split_tf32(v.x, hi.x, lo.x);
-          split_tf32(v.y, hi.y, lo.y);
-          split_tf32(v.z, hi.z, lo.z);
-          split_tf32(v.w, hi.w, lo.w);
+          split_tf32(v[i].x, hi.x, lo.x);
+          split_tf32(v[i].y, hi.y, lo.y);
+          split_tf32(v[i].z, hi.z, lo.z);
+          split_tf32(v[i].w, hi.w, lo.w);
           *reinterpret_cast<float4*>(dst + i * XR * 128) = hi;
-          *reinterpret_cast<float4*>(dst + XA * x_atom + i * XR * 128) = lo;
+          *reinterpret_cast<float4*>(dst + x_atom + i * XR * 128) = lo;
         }
       }
       if (PX == 2 || !(by_tma >> xr.slot & 1)) {
@@ -507,13 +517,13 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&xfull[xr.slot]);
       }
-      xr.next(p.x_slots);
+      step(xr);
       --pending;
       issue();
     }
     cp_async_wait<0>();
     // given up: loads in flight land before the CTA's shared memory is released
-    for (; !ok && pending > 0; --pending, xr.next(p.x_slots))
+    for (; !ok && pending > 0; --pending, step(xr))
       mbar_wait_drain(PX == 2 ? &xraw[xr.slot] : &xfull[xr.slot], xr.parity);
   } else if (warp < kWarpT) {
     // ---------------- epilogue: base + accumulators -> y ----------------
@@ -790,42 +800,29 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             ok = stage_wait(&xfull[xr.slot], xr.parity, abort_flag, err, 32u);
             tc_fence_after();
             const uint32_t x0 = desc_lo(smem_u32(sX) + xr.slot * x_slot);
-            // a piece of A against x: `at` its 128-byte rows, `low` all but its first part
-            auto piece = [&](int at, bool low, bool first) {
+            auto piece = [&](int part) {  // a part of A against x
               if (!ok) return;
               ok = stage_wait(&afull[ar.slot], ar.parity, abort_flag, err, 64u);
               if (!ok) return;
               tc_fence_after();
-              const uint32_t x = x0 + at * (x_atom >> 4), w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
-              if (!low) {
+              const uint32_t w = desc_lo(smem_u32(sA) + ar.slot * a_slot);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                  const uint32_t on = s > 0 || at > 0 ? 1 : more;
-                  if (PX == 2) {
-                    umma_tf32(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, on);
-                    umma_tf32(acc_lo, desc_at(x + (x_atom >> 3) + 2 * s), desc_at(w + 2 * s), id,
-                              s > 0 || at > 0 ? 1 : c > 0);
-                  } else {
-                    umma_f16(acc, desc_at(x + 2 * s), desc_at(w + 2 * s), id, on);
-                  }
-                }
-              } else {
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                  if (PX == 2) umma_tf32(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, 1);
-                  else umma_f16(acc_lo, desc_at(x + 2 * s), desc_at(w + 2 * s), id, s > 0 || !first ? 1 : c > 0);
+              for (int s = 0; s < 4; ++s) {
+                const uint64_t dx = desc_at(x0 + 2 * s), dw = desc_at(w + 2 * s);
+                const uint32_t on = s > 0 || c > 0;  // the low parts' accumulator has something
+                if (PX == 2) {
+                  umma_tf32(part == 0 ? acc : acc_lo, dx, dw, id, part > 0 ? 1 : s > 0 ? 1 : more);
+                  if (part == 0) umma_tf32(acc_lo, desc_at(x0 + (x_atom >> 4) + 2 * s), dw, id, on);
+                } else {
+                  umma_f16(part == 0 ? acc : acc_lo, dx, dw, id, part > 1 ? 1 : part == 1 ? on : s > 0 ? 1 : more);
                 }
               }
               umma_commit(&aempty[ar.slot]);
               ar.next(p.a_slots);
             };
-            piece(0, false, true);
-            if (PX == 2) piece(1, false, true);
-            if (PA > 1) {
-              piece(0, true, true);
-              if (PX == 2) piece(1, true, true);
-              if (PX == 1 && PA > 2) piece(0, true, false);
-            }
+            piece(0);
+            if (PA > 1) piece(1);
+            if (PX == 1 && PA > 2) piece(2);
             more = 1;
             if (!ok) break;
             umma_commit(&xempty[xr.slot]);
@@ -933,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int rcs = (un.rp + KC - 1) / KC;
       const uint32_t bytes = is_a ? un.rank * 128 : kBPlane;  // of a piece
       const uint8_t* src = is_a ? un.ta : un.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
-      for (int n = is_a ? k_stages * XA * PA : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
+      for (int n = is_a ? k_stages * PA : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
         ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
         if (!ok) break;
         mbar_arrive_expect_tx(&full[r.slot], bytes);
@@ -955,7 +952,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 
 // The bank's weights as the kernel's tiles, tf32 planes (hi, and lo for float32
 // weights) of rows of 32 values whose 16-byte pieces are swizzled by the row
-// number; zeros outside. A: [k stage][plane][2 x 32 channels][rank rows]. B:
+// number; zeros outside. A: [32 channels][plane][rank rows]. B:
 // [chunk of 256 channels][even, odd][32 ranks][plane][128 rows], row i of a
 // chunk's tile g being channel 2 i + g.
 template <class WT>
@@ -972,9 +969,8 @@ __global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int
       row = (int)(i / ka);
       const int kk = (int)(i % ka);
       c = kk % KC;
-      const int64_t atom = (int64_t)ad.rank * 128;
-      plane = 2 * atom;
-      tile = const_cast<uint8_t*>(ad.ta[kDtF32]) + (int64_t)(kk / KS) * planes * plane + kk % KS / KC * atom;
+      plane = (int64_t)ad.rank * 128;
+      tile = const_cast<uint8_t*>(ad.ta[kDtF32]) + (int64_t)(kk / KC) * planes * plane;
       if (kk < k_in) v = as_f32(static_cast<const WT*>(ad.a)[i]);
     } else {
       const int64_t b = i - na, t = b / (128 * KC);
@@ -1016,8 +1012,8 @@ __global__ void lowrank_tiles16_kernel(LowRankAdapter ad, int k_in, int ka, int 
   if (ad.unscale && top > 0.0f && top < __uint_as_float(0x7f800000u)) up = min(13 - ilogbf(top), 100);
   if (ad.unscale && threadIdx.x == 0) const_cast<float*>(ad.unscale)[j] = ldexpf(1.0f, -up);
   auto put = [&](int xtype, int parts, int part, int k, uint16_t bits) {
-    uint8_t* row = const_cast<uint8_t*>(ad.ta[xtype]) + ((int64_t)(k / KS * parts + part) * ad.rank + j) * 128;
-    const int c = k % KS;
+    uint8_t* row = const_cast<uint8_t*>(ad.ta[xtype]) + ((int64_t)(k / 64 * parts + part) * ad.rank + j) * 128;
+    const int c = k % 64;
     *reinterpret_cast<uint16_t*>(row + (((c >> 3) ^ (j & 7)) * 16) + (c & 7) * 2) = bits;
   };
   for (int k = threadIdx.x; k < ka; k += blockDim.x) {
@@ -1041,7 +1037,7 @@ __global__ void lowrank_tiles16_kernel(LowRankAdapter ad, int k_in, int ka, int 
 
 template <class XT, class YT>
 cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
-  constexpr int XTYPE = dtype_of<XT>(), PX = XTYPE == kDtF32 ? 2 : 1, XA = PX;
+  constexpr int XTYPE = dtype_of<XT>(), PX = XTYPE == kDtF32 ? 2 : 1;
   const int chunks = (p.bank.n_out + 255) / 256;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1055,7 +1051,7 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = (p.bank.max_rank + 15) / 16 * 16 * 128;
   int smem = 0;
   for (; p.rt >= 16; p.rt /= 2) {
-    const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * XA * p.rt * 128;
+    const int t_buf = t_chunks * 2 * p.rt * 128, x_slot = PX * p.rt * 128;
     int left = kMaxSmem - 1024 - kMiscBytes - kEpiWarps * 2048 - 2 * (kBPlane + a_slot + x_slot) - t_buf;
     if (left < 0) continue;
     p.t_bufs = 1, p.a_slots = p.b_slots = p.x_slots = 2, p.epi_ring = 2048;
@@ -1064,12 +1060,13 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
       left -= bytes, n += by;
       return true;
     };
-    grow(p.x_slots, 1, 3, x_slot);
+    while (grow(p.x_slots, 2, 6, 2 * x_slot)) {
+    }
     grow(p.epi_ring, 2048, 4096, kEpiWarps * 2048);
     for (bool any = true; any;) {
       any = grow(p.b_slots, 1, kMaxSlots, kBPlane);
       any |= grow(p.a_slots, 1, kMaxSlots, a_slot);
-      any |= grow(p.x_slots, 1, 6, x_slot);
+      any |= grow(p.x_slots, 2, kMaxSlots, 2 * x_slot);
       any |= grow(p.t_bufs, 1, 2, t_buf);
     }
     smem = kMaxSmem - left;
@@ -1107,7 +1104,7 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
 }  // namespace
 
 size_t lowrank_tile_bytes_a(int rank, int ka, int wtype, int xtype) {
-  return (size_t)(ka / (xtype == kDtF32 ? KC : KS)) * rank * 128 * a_parts(xtype, wtype);
+  return (size_t)(ka / (xtype == kDtF32 ? KC : 64)) * rank * 128 * a_parts(xtype, wtype);
 }
 size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype) {
   return (size_t)((n_out + 255) / 256 * 2) * ((rp + KC - 1) / KC) * kBPlane * (wtype == kDtF32 ? 2 : 1);
