@@ -66,7 +66,6 @@ static_assert(kRt == kAdapterTileRows && kRt <= kTWarps * 32, "a unit is a tile 
 constexpr int kMaxSlots = 8;
 constexpr int kBPlane = 128 * 128;  // one plane of a slot of B: 128 channels x 128 bytes
 constexpr int kMiscBytes = 1792;
-constexpr int kEpiRows = 8;  // rows per batch of an epilogue warp's ring of base
 constexpr int kMaxSmem = 232448;  // an MMA reads 128 rows from a slot's start: a short slot's run on into sW and sT
 
 __device__ uint32_t g_lowrank_error;
@@ -76,8 +75,8 @@ __host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) {
   return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // One lane of a converged warp. Unlike a test of the lane number it tells the
-// compiler that a single thread goes on, which the operands of an MMA need: 30
-// instead of 110 cycles to issue one.
+// compiler that a single thread goes on, which the operands of an MMA or a TMA
+// copy need: 30 instead of 110 cycles to issue an MMA.
 __device__ __forceinline__ bool elect_lane() {
   uint32_t p;
   asm volatile(
@@ -251,8 +250,12 @@ __host__ __device__ constexpr int dtype_of() {
   return std::is_same<XT, float>::value ? kDtF32 : std::is_same<XT, __half>::value ? kDtF16 : kDtBF16;
 }
 
+// Rows per batch of base that an epilogue warp copies (its registers hold eight at a time).
+template <class YT>
+__host__ __device__ constexpr int epi_rows() { return sizeof(YT) == 4 ? 8 : 16; }
+
 struct TcParams {
-  CUtensorMap tm_x, tm_b;  // rows of x (boxes of rt rows x 128 bytes, swizzled) and of base (8 rows x 64 channels)
+  CUtensorMap tm_x, tm_b;  // rows of x (boxes of rt rows x 128 bytes, swizzled) and of base (a batch x 64 channels)
   LowRankBank bank;
   AdapterPlanDev plan;
   LowRankArgs a;
@@ -447,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           by_tma |= 1u << ir.slot;
           // float32: the X warps take over when the bytes are there; 16-bit: they go straight to the MMAs
           uint64_t* bar = PX == 2 ? &xraw[ir.slot] : &xfull[ir.slot];
-          if (lane == 0) {
+          if (elect_lane()) {
             if (warp == first_warp) {
               mbar_arrive_expect_tx(bar, x_atom);
               tma_load_2d(&p.tm_x, bar, dst, ks * KS, tma_row);
@@ -529,14 +532,15 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     // ---------------- epilogue: base + accumulators -> y ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
-    constexpr int B = kEpiRows, RB = 64 * sizeof(YT);     // bytes of a row in the ring: this warp's 64 channels
+    constexpr int B = epi_rows<YT>(), RB = 64 * sizeof(YT);  // rows of a batch, bytes of one: this warp's 64 channels
+    constexpr int S = 8;                                     // rows in registers
     const int nb = p.epi_ring / (B * RB);                 // batches: 1 to 4
     const YT* base = static_cast<const YT*>(p.a.base);
     YT* y = static_cast<YT*>(p.a.y);
     const int quarter = warp & 3, n_out = p.bank.n_out;
     const uint32_t ring = smem_u32(sE) + (warp - kWarpEpi) * p.epi_ring;
     // this warp's rows [i0, i1) of a unit: a fourth of them, eight at least
-    const int per = max(B, p.rt / 4), i0 = ((warp - kWarpEpi) >> 2) * per;
+    const int per = max(S, p.rt / 4), i0 = ((warp - kWarpEpi) >> 2) * per;
     // the cursor of the copies: a unit, chunk fc of [.., fc1), rows from fi. The rows follow each other from frow0
     // (that of row i0), or lane i holds row i0 + i.
     UnitCursor fu, uc;
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         };
         const uint32_t fslot = ring + fr.slot * (B * RB);
         const bool tma = p.b_copy == 16 && frow0 >= 0 && fi + B <= fi1;  // a box holds rows of the unit only
-        if (lane == 0) {
+        if (elect_lane()) {
           if (tma) {
             mbar_arrive_expect_tx(&bars[fr.slot], B * RB);
             tma_load_2d(&p.tm_b, &bars[fr.slot], sE + (fslot - smem_u32(sE)), ch, frow0 + fi - i0);
@@ -604,15 +608,18 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         } else if constexpr (sizeof(YT) == 2) {  // odd 16-bit addresses: loads, clamped instead of conditional
           const YT* c0 = base + min(ch + lane, n_out - 1);
           const YT* c1 = base + min(ch + lane + 32, n_out - 1);
-          YT v0[B], v1[B];
-#pragma unroll
-          for (int r = 0; r < B; ++r) {
-            const int64_t o = row_of(r) * p.a.ldb;
-            v0[r] = c0[o], v1[r] = c1[o];
-          }
           YT* dst = reinterpret_cast<YT*>(sE + (fslot - smem_u32(sE)));
+#pragma unroll 1
+          for (int r = 0; r < B; r += 4) {
+            YT v0[4], v1[4];
 #pragma unroll
-          for (int r = 0; r < B; ++r) dst[r * 64 + lane] = v0[r], dst[r * 64 + lane + 32] = v1[r];
+            for (int j = 0; j < 4; ++j) {
+              const int64_t o = row_of(r + j) * p.a.ldb;
+              v0[j] = c0[o], v1[j] = c1[o];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[(r + j) * 64 + lane] = v0[j], dst[(r + j) * 64 + lane + 32] = v1[j];
+          }
         }
         fr.next(nb);
         fi += B;
@@ -650,45 +657,50 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         tc_fence_after();
         const int ch = c * 256 + quarter * 64 + lane * 2;
         const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (d & 1) * 128u;
-        for (int i = i0; i < i1; i += B) {
-          Pair b[B];
+        for (int i = i0; i < i1; i += S) {
+          Pair b[S];
+          const int sub = (i - i0) % B;  // rows of the batch before these
           if (base) {
-            if (!filled) fill();  // the cursor was at its limit
-            copy_wait(filled - 1);
-            ok = warp_wait(&bars[er.slot], er.parity, abort_flag, err, 32768u);
-            if (!ok) break;
-            __syncwarp();  // the other lanes' copies
-            const uint8_t* src = sE + (ring - smem_u32(sE)) + er.slot * (B * RB) + lane * 2 * sizeof(YT);
+            if (sub == 0) {
+              if (!filled) fill();  // the cursor was at its limit
+              copy_wait(filled - 1);
+              ok = warp_wait(&bars[er.slot], er.parity, abort_flag, err, 32768u);
+              if (!ok) break;
+              __syncwarp();  // the other lanes' copies
+            }
+            const uint8_t* src = sE + (ring - smem_u32(sE)) + (er.slot * B + sub) * RB + lane * 2 * sizeof(YT);
 #pragma unroll
-            for (int j = 0; j < B; ++j) b[j] = *reinterpret_cast<const Pair*>(src + j * RB);
-            er.next(nb);
-            --filled;
-            __syncwarp();
-            fill();
+            for (int j = 0; j < S; ++j) b[j] = *reinterpret_cast<const Pair*>(src + j * RB);
+            if (sub + S == B || i + S >= i1) {
+              er.next(nb);
+              --filled;
+              __syncwarp();
+              fill();
+            }
           } else {
 #pragma unroll
-            for (int j = 0; j < B; ++j) b[j].e[0] = b[j].e[1] = as_type<YT>(0.0f);
+            for (int j = 0; j < S; ++j) b[j].e[0] = b[j].e[1] = as_type<YT>(0.0f);
           }
-          uint32_t v0[B], v1[B];
+          uint32_t v0[S], v1[S];
           tmem_ld8(acc + (uint32_t)i, v0);
           tmem_ld8(acc + (uint32_t)(p.rt + i), v1);
           tmem_wait_ld();
           reg_barrier8(v0);
           reg_barrier8(v1);
 #pragma unroll
-          for (int j = 0; j < B; ++j) {
+          for (int j = 0; j < S; ++j) {
             b[j].e[0] = as_type<YT>(__fadd_rn(as_f32(b[j].e[0]), __uint_as_float(v0[j])));
             b[j].e[1] = as_type<YT>(__fadd_rn(as_f32(b[j].e[1]), __uint_as_float(v1[j])));
           }
-          if (p.y_pair && un.row0 >= 0 && i + B <= i1) {  // the usual case in few instructions
+          if (p.y_pair && un.row0 >= 0 && i + S <= i1) {  // the usual case in few instructions
             if (ch < n_out) {
               YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + ch;
 #pragma unroll
-              for (int j = 0; j < B; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
+              for (int j = 0; j < S; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
+            for (int j = 0; j < S; ++j) {
               const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
               if (i + j >= i1) continue;
               YT* dst = y + (int64_t)row * p.a.ldy + ch;
@@ -914,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       }
       if (last) break;
     }
-  } else if (warp <= kWarpB && lane == 0) {
+  } else if (warp <= kWarpB && elect_lane()) {
     // ---------------- weights: bulk copies of the bank's tiles (A's, or B's) ----------------
     const bool is_a = warp == kWarpA;
     uint8_t* ring = is_a ? sA : sB;
@@ -1092,7 +1104,7 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   if (p.x_vec)
     e = map(&p.tm_x, p.a.x, XTYPE, p.bank.k_in, p.a.ldx, 128 / sizeof(XT), p.rt, CU_TENSOR_MAP_SWIZZLE_128B);
   if (e == cudaSuccess && base && p.b_copy == 16)
-    e = map(&p.tm_b, p.a.base, dtype_of<YT>(), p.bank.n_out, p.a.ldb, 64, kEpiRows, CU_TENSOR_MAP_SWIZZLE_NONE);
+    e = map(&p.tm_b, p.a.base, dtype_of<YT>(), p.bank.n_out, p.a.ldb, 64, epi_rows<YT>(), CU_TENSOR_MAP_SWIZZLE_NONE);
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(lowrank_tc_kernel<XT, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
