@@ -88,6 +88,7 @@ _SIGNATURES = {
                                     C.c_void_p, C.c_int32, C.c_int64, C.c_void_p]),
     "sem_lowrank_apply_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                                          C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sem_lowrank_path": (C.c_int, [C.c_int32]),
     "sem_lowrank_check": (C.c_int, [C.c_void_p]),
     "sem_block_norm_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_int32,
                                         C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),

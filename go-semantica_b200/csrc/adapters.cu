@@ -69,159 +69,265 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
   *reinterpret_cast<Pack*>(p) = k;
 }
 
-// Eight consecutive weights (16-byte aligned) of a bank's type.
-__device__ __forceinline__ void load_weights8(const void* base, int64_t at, int wtype, float (&v)[8]) {
-  if (wtype == kDtF32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else if (wtype == kDtF16) {
-    load_vec<8>(static_cast<const __half*>(base) + at, v);
+// Eight consecutive weights (16-byte aligned) in two steps, so that the loads are on their way while other work
+// is done: the bytes, then the values. WT: float, or any 16-bit type (bf16 or
+// fp16 by wtype).
+template <class WT>
+struct RawWeights8 {
+  uint4 q[sizeof(WT) == 4 ? 2 : 1];
+};
+template <class WT>
+__device__ __forceinline__ void fetch_weights8(const void* base, int64_t at, RawWeights8<WT>& r) {
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const WT*>(base) + at);
+  r.q[0] = p[0];
+  if constexpr (sizeof(WT) == 4) r.q[1] = p[1];
+}
+template <class WT>
+__device__ __forceinline__ void weights8(const RawWeights8<WT>& r, int wtype, float (&v)[8]) {
+  if constexpr (sizeof(WT) == 4) {
+    const uint32_t w[8] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w, r.q[1].x, r.q[1].y, r.q[1].z, r.q[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
   } else {
-    load_vec<8>(static_cast<const __nv_bfloat16*>(base) + at, v);
+    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+    if (wtype == kDtBF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Low-rank adapters on CUDA cores
 // ---------------------------------------------------------------------------
-// A cluster of eight CTAs takes one tile: CTA c sums its eighth of the input
-// channels into partial t = x A^T (16 rows at a time), the partials meet
-// through distributed shared memory, every CTA adds them in the same order
-// (results do not depend on timing), and each finishes its eighth of the
-// output channels. One launch with no workspace: a single row's latency is two
-// short dependent loads (A, then B) instead of one SM walking both weights.
-constexpr int kSmallCtas = 8, kSmallThreads = 256, kSmallWarps = kSmallThreads / 32;
-constexpr int kSmallChunk = 128;  // input channels staged at a time, 4 per lane
+// A unit is up to 16 rows of one adapter. A cluster of two, four or eight CTAs
+// takes it: each CTA sums its share of the input channels into a partial t =
+// x A^T and writes it to every CTA of the cluster (distributed shared memory);
+// after one cluster barrier each adds the partials in the same order and
+// finishes its share of the output channels. One launch, no workspace, and two
+// short dependent load phases (A, then B, which is fetched before the barrier
+// with base) where one SM would walk both weights: what a few rows cost is
+// latency. The shares do not go by the batch (a row's sums are the same for
+// any cluster size: the input channels are cut in eight, and a CTA of a
+// smaller cluster sums several of the eight one after the other). Float32 FMA
+// throughout.
+constexpr int kSmallParts = 8, kSmallThreads = 256, kSmallWarps = kSmallThreads / 32;
+constexpr int kSmallChunk = 128, kSmallLd = kSmallChunk + 4;  // input channels staged at a time, padded (banks)
+constexpr int kSmallRows = kAdapterSmallRows;
+static_assert(kSmallRows == 16, "a thread's row is its lane modulo 16");
 
-template <class XT, class YT>
-__global__ void __cluster_dims__(kSmallCtas, 1, 1) __launch_bounds__(kSmallThreads)
-    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, LowRankArgs a) {
-  constexpr int R = kAdapterSmallRows;
-  __shared__ __align__(16) float s_x[R][kSmallChunk];
-  __shared__ __align__(16) float s_part[kLowRankMaxRank][R];
-  __shared__ __align__(16) float s_t[kLowRankMaxRank][R];
-  __shared__ int32_t s_row[R];
-  __shared__ float s_scale[R];
+inline __host__ __device__ int small_smem_floats(int max_rank) {  // x, A, the partials of two units in turn, t
+  return (kSmallRows + max_rank) * kSmallLd + 2 * kSmallParts * kSmallRows * max_rank + kSmallRows * ((max_rank + 7) & ~7);
+}
+
+// Eight consecutive values, of which those from `n` on are zero; `vec`: 16-byte
+// aligned in memory (all of it is read then only if n >= 8).
+template <class T>
+__device__ __forceinline__ void load_row8(const T* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      load_vec<8>(p, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+// RU: ranks per warp at most (ranks up to 8 RU).
+template <class XT, class YT, class WT, int RU>
+__global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
+    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, int large_too, LowRankArgs a, int x_vec) {
+  extern __shared__ __align__(16) float smem[];
+  float* s_x = smem;                                   // [16][kSmallLd]
+  float* s_a = s_x + kSmallRows * kSmallLd;            // [rank][kSmallLd]
+  float* s_part = s_a + bank.max_rank * kSmallLd;      // [2][eighth][16 * rank]
+  float* s_t = s_part + 2 * kSmallParts * kSmallRows * bank.max_rank;  // [rank][16]
+  __shared__ int32_t s_row[kSmallRows];
+  __shared__ float s_scale[kSmallRows];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank_id = (int)cluster.block_rank();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n_tiles = plan.counts[1];
+  const int cta = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const XT* x = static_cast<const XT*>(a.x);
   const YT* base = static_cast<const YT*>(a.base);
   YT* y = static_cast<YT*>(a.y);
-  // this CTA's input and output channels
-  const int kper = (bank.ka / 32 + kSmallCtas - 1) / kSmallCtas * 32;
-  const int k0 = min(bank.k_in, rank_id * kper), k1 = min(bank.k_in, k0 + kper);
-  const int nper = (bank.n_out + kSmallCtas - 1) / kSmallCtas;
-  const int n0 = min(bank.n_out, rank_id * nper), n1 = min(bank.n_out, n0 + nper);
+  // an eighth of the input channels (a multiple of 8), this CTA's output channels (an even number)
+  const int kper = ((bank.k_in + kSmallParts - 1) / kSmallParts + 7) & ~7;
+  const int nper = ((bank.n_out + ctas - 1) / ctas + 1) & ~1;
+  const int n0 = min(bank.n_out, cta * nper), n1 = min(bank.n_out, n0 + nper);
+  constexpr int kSubs = kAdapterTileRows / kSmallRows;  // units of a large tile
+  const bool in_place = a.base == a.y && a.ldb == a.ldy;
+  int set = 0;
+  bool started = false;  // every CTA of the cluster runs: its shared memory can be written
+  cluster.barrier_arrive();
+  const AdapterTile first = plan.small[min((int)(blockIdx.x / ctas), plan.max_seqs)];  // without waiting for the count
+  const int n_small = plan.counts[1], n_units = n_small + (large_too ? plan.counts[0] * kSubs : 0);
 
-  for (int tile = (int)(blockIdx.x / kSmallCtas); tile < n_tiles; tile += (int)(gridDim.x / kSmallCtas)) {
-    const AdapterTile tl = plan.small[tile];
+  for (int u = (int)(blockIdx.x / ctas); u < n_units; u += (int)(gridDim.x / ctas)) {
+    AdapterTile tl = first;
+    int sub = 0;
+    if (u >= n_small) {
+      tl = plan.large[(u - n_small) / kSubs];
+      sub = (u - n_small) % kSubs * kSmallRows;
+    } else if (u != (int)(blockIdx.x / ctas)) {
+      tl = plan.small[u];
+    }
+    const int rows = min(kSmallRows, tl.rows - sub);
+    if (rows <= 0) continue;  // the whole cluster
     LowRankAdapter ad{};
     if (tl.adapter >= 0 && tl.adapter < bank.n_adapters) ad = bank.adapters[tl.adapter];
-    if (ad.rank == 0 && a.base == a.y && a.ldb == a.ldy) continue;  // in place and nothing to add (the whole cluster)
-    for (int sub = 0; sub < tl.rows; sub += R) {
-      const int rows = min(R, tl.rows - sub);
-      if (tid < R) {
-        const int p = tl.pos0 + sub + min(tid, rows - 1);
-        s_row[tid] = plan.pos_row[p];
-        float sc = ad.scale;
-        if (a.absmax) sc = __fmul_rn(sc, __fdiv_rn(__uint_as_float(a.absmax[a.per_seq ? plan.pos_seq[p] : 0]), 127.0f));
-        s_scale[tid] = sc;
+    if (ad.rank == 0 && in_place) continue;  // nothing to add (the whole cluster)
+    __syncthreads();  // the previous unit's rows, scales and t are read
+    if (tid < kSmallRows) {
+      const int r = sub + min(tid, rows - 1);  // rows behind the last one repeat it and are not stored
+      s_row[tid] = tl.row0 >= 0 ? tl.row0 + r : plan.pos_row[tl.pos0 + r];
+      float sc = ad.scale;
+      if (a.absmax)
+        sc = __fmul_rn(sc, __fdiv_rn(__uint_as_float(a.absmax[a.per_seq ? plan.pos_seq[tl.pos0 + r] : 0]), 127.0f));
+      s_scale[tid] = sc;
+    }
+    __syncthreads();
+    float* part = s_part + set * kSmallParts * kSmallRows * bank.max_rank;
+    set ^= 1;
+    const int size = ad.rank * kSmallRows;
+    // a thread: four rows of a pair of output channels; base and the first ranks of B are on their way while t is summed
+    const int items = (n1 - n0 + 1) / 2 * (kSmallRows / 4);
+    const int q = tid & 3;  // its rows 4 q ..
+    YT b[2][4];
+    RawWeights8<WT> w[2];
+    auto fetch = [&](int item) {
+      const int ch = n0 + item / 4 * 2;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = min(ch + e, n1 - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          b[e][i] = base ? base[(int64_t)s_row[q * 4 + i] * a.ldb + c] : from_f32<YT>(0.0f);
+        if (ad.rank > 0) fetch_weights8(ad.b, (int64_t)c * ad.rp, w[e]);
       }
-      __syncthreads();
-      if (ad.rank > 0) {
-        // partial t of this CTA's input channels: a warp per rank row j, its
-        // lanes four channels each, 16 rows of x from shared memory
-        for (int j0 = 0; j0 < ad.rank; j0 += kSmallWarps * 4) {
-          float acc[4][R];
+    };
+    if (tid < items) fetch(tid);
+    if (ad.rank > 0) {
+      // a thread: one row (lane % 16), half of each chunk's channels (lane / 16), every eighth rank
+      for (int eighth = cta; eighth < kSmallParts; eighth += ctas) {
+        const int k0 = min(bank.k_in, eighth * kper), k1 = min(bank.k_in, k0 + kper);
+        float acc[RU];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int i = 0; i < R; ++i) acc[u][i] = 0.0f;
-          for (int kc = k0; kc < k1; kc += kSmallChunk) {
-            const int kn = min(kSmallChunk, k1 - kc);
-            __syncthreads();
-            for (int i = tid; i < R * kSmallChunk; i += kSmallThreads) {
-              const int r = i / kSmallChunk, c = i % kSmallChunk;
-              s_x[r][c] = r < rows && c < kn ? to_f32(x[(int64_t)s_row[r] * a.ldx + kc + c]) : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int j = j0 + warp + u * kSmallWarps;
-              if (j >= ad.rank || kc + lane * 4 >= bank.ka) continue;  // A's rows end at ka (zeros behind k_in)
-              float w[4];
-              const int64_t at = (int64_t)j * bank.ka + kc + lane * 4;
-              if (bank.wtype == kDtF32) load_vec<4>(static_cast<const float*>(ad.a) + at, w);
-              else if (bank.wtype == kDtF16) load_vec<4>(static_cast<const __half*>(ad.a) + at, w);
-              else load_vec<4>(static_cast<const __nv_bfloat16*>(ad.a) + at, w);
-              if (lane * 4 >= kn) w[0] = w[1] = w[2] = w[3] = 0.0f;  // the next CTA's channels
-#pragma unroll
-              for (int i = 0; i < R; ++i) {
-                const float4 v = *reinterpret_cast<const float4*>(&s_x[i][lane * 4]);
-                acc[u][i] = fmaf(v.x, w[0], fmaf(v.y, w[1], fmaf(v.z, w[2], fmaf(v.w, w[3], acc[u][i]))));
-              }
-            }
+        for (int i = 0; i < RU; ++i) acc[i] = 0.0f;
+        for (int kc = k0; kc < k1; kc += kSmallChunk) {
+          const int kn = min(kSmallChunk, k1 - kc), oct = (kn + 7) / 8;
+          if (eighth != cta || kc > k0) __syncthreads();
+          auto put = [&](int r, int c, const float (&v)[8]) {
+            float4* d = reinterpret_cast<float4*>(s_x + r * kSmallLd + c);
+            d[0] = make_float4(v[0], v[1], v[2], v[3]);
+            d[1] = make_float4(v[4], v[5], v[6], v[7]);
+          };
+          // x is one piece per thread at most; the first of A's is loaded before it is waited for
+          const int r = tid / oct, c = tid % oct * 8;
+          float vx[8], va[8];
+          auto load_a = [&](int j, int ca) {  // zeros behind k_in
+            RawWeights8<WT> raw;
+            fetch_weights8(ad.a, (int64_t)j * bank.ka + kc + ca, raw);
+            weights8(raw, bank.wtype, va);
+          };
+          if (r < kSmallRows) load_row8(x + (int64_t)s_row[r] * a.ldx + kc + c, kn - c, x_vec != 0, vx);
+          if (r < ad.rank) load_a(r, c);
+          if (r < kSmallRows) put(r, c, vx);
+          if (r < ad.rank) put(kSmallRows + r, c, va);
+          for (int i = tid + kSmallThreads; i < ad.rank * oct; i += kSmallThreads) {
+            load_a(i / oct, i % oct * 8);
+            put(kSmallRows + i / oct, i % oct * 8, va);
           }
+          __syncthreads();
+          const float* xr = s_x + (lane & 15) * kSmallLd;
+#pragma unroll 4
+          for (int c = (lane >> 4) * 4; c < oct * 8; c += 8) {
+            const float4 v = *reinterpret_cast<const float4*>(xr + c);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int j = j0 + warp + u * kSmallWarps;
-            if (j >= ad.rank) continue;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              float v = acc[u][i];
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
-              if (lane == i) s_part[j][i] = v;
+            for (int i = 0; i < RU; ++i) {  // ranks there are not: the last one again
+              const float4 w4 = *reinterpret_cast<const float4*>(s_a + min(warp + i * kSmallWarps, ad.rank - 1) * kSmallLd + c);
+              acc[i] = fmaf(v.x, w4.x, fmaf(v.y, w4.y, fmaf(v.z, w4.z, fmaf(v.w, w4.w, acc[i]))));
             }
           }
         }
-        cluster.sync();
-        for (int i = tid; i < ad.rank * R; i += kSmallThreads) {
-          float v = 0.0f;
+        if (!started) cluster.barrier_wait();
+        started = true;
 #pragma unroll
-          for (int c = 0; c < kSmallCtas; ++c)
-            v = __fadd_rn(v, *cluster.map_shared_rank(&s_part[0][0] + i, c));
-          (&s_t[0][0])[i] = __fmul_rn(v, s_scale[i % R]);
+        for (int i = 0; i < RU; ++i) {
+          const int j = warp + i * kSmallWarps;
+          if (j >= ad.rank) break;
+          const float v = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 16));
+          // both halves of the lanes hold the sum: each sends it to half of the CTAs
+          float* mine = part + eighth * size + j * kSmallRows + (lane & 15);
+          for (int d = lane >> 4; d < ctas; d += 2) *cluster.map_shared_rank(mine, d) = v;
         }
-        cluster.sync();  // the partials are free for the next 16 rows
       }
-      // this CTA's output channels: a thread per (channel, half of the rows)
-      constexpr int H = R / 2;
-      const int half = tid & 1;
-      for (int n = n0 + (tid >> 1); n < n1; n += kSmallThreads / 2) {
-        float acc[H];
+    }
+    if (ad.rank > 0) {
+      cluster.sync();
+      for (int i = tid; i < ad.rp * kSmallRows; i += kSmallThreads) {
+        float v = 0.0f;
+        if (i < size) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) acc[i] = 0.0f;
-        for (int j = 0; j < ad.rank; j += 8) {  // B's columns end at rp, zeros behind the rank
-          float w[8];
-          load_weights8(ad.b, (int64_t)n * ad.rp + j, bank.wtype, w);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            if (j + u >= ad.rank) break;
-#pragma unroll
-            for (int i = 0; i < H; i += 4) {
-              const float4 t = *reinterpret_cast<const float4*>(&s_t[j + u][half * H + i]);
-              acc[i] = fmaf(t.x, w[u], acc[i]);
-              acc[i + 1] = fmaf(t.y, w[u], acc[i + 1]);
-              acc[i + 2] = fmaf(t.z, w[u], acc[i + 2]);
-              acc[i + 3] = fmaf(t.w, w[u], acc[i + 3]);
-            }
-          }
+          for (int c = 0; c < kSmallParts; ++c) v = __fadd_rn(v, part[c * size + i]);
+          v = __fmul_rn(v, s_scale[i & 15]);
         }
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          const int r = half * H + i;
-          if (r >= rows) continue;
-          const float b = base ? to_f32(base[(int64_t)s_row[r] * a.ldb + n]) : 0.0f;
-          y[(int64_t)s_row[r] * a.ldy + n] = from_f32<YT>(__fadd_rn(b, acc[i]));
-        }
+        s_t[i] = v;  // zeros for the columns of B behind the rank
       }
       __syncthreads();
     }
+    for (int item = tid; item < items; item += kSmallThreads) {
+      if (item != tid) fetch(item);
+      const int ch = n0 + item / 4 * 2;
+      float o[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[0][i] = o[1][i] = 0.0f;
+      for (int j = 0; j < ad.rp; j += 8) {
+        RawWeights8<WT> nw[2];
+        if (j + 8 < ad.rp) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            fetch_weights8(ad.b, (int64_t)min(ch + e, n1 - 1) * ad.rp + j + 8, nw[e]);
+        }
+        float f[2][8];
+        weights8(w[0], bank.wtype, f[0]);
+        weights8(w[1], bank.wtype, f[1]);
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          const float4 t = *reinterpret_cast<const float4*>(s_t + (j + v) * kSmallRows + q * 4);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            o[e][0] = fmaf(t.x, f[e][v], o[e][0]);
+            o[e][1] = fmaf(t.y, f[e][v], o[e][1]);
+            o[e][2] = fmaf(t.z, f[e][v], o[e][2]);
+            o[e][3] = fmaf(t.w, f[e][v], o[e][3]);
+          }
+        }
+        w[0] = nw[0], w[1] = nw[1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (q * 4 + i >= rows) break;
+        YT* d = y + (int64_t)s_row[q * 4 + i] * a.ldy + ch;
+        d[0] = from_f32<YT>(__fadd_rn(to_f32(b[0][i]), o[0][i]));
+        if (ch + 1 < n1) d[1] = from_f32<YT>(__fadd_rn(to_f32(b[1][i]), o[1][i]));
+      }
+    }
   }
+  if (!started) cluster.barrier_wait();
+  cluster.sync();  // no CTA leaves while another may still write to it
 }
 
 // ---------------------------------------------------------------------------
@@ -336,19 +442,16 @@ __global__ void __launch_bounds__(TPR > kNormThreads ? TPR : kNormThreads) block
 template <class OT, class HT, int TPR, int VEC>
 cudaError_t norm_chunks(const BlockNormArgs& a, cudaStream_t st) {
   constexpr int kThreads = TPR > kNormThreads ? TPR : kNormThreads;
-  constexpr int kRows = kThreads / TPR, kMost = 32 / VEC;  // 32 elements per thread at most
+  constexpr int kRows = kThreads / TPR;
+  constexpr int kMost = (VEC == 1 && TPR < 512 ? 16 : 32) / VEC;  // elements per thread at most: 32, or 16 single ones
   const int64_t grid = (a.rows + kRows - 1) / kRows;
   const int nc = ((a.dim + VEC - 1) / VEC + TPR - 1) / TPR;
   if (nc > kMost || grid > 0x7fffffff) return cudaErrorInvalidValue;
-  if constexpr (VEC == 1) {
-    block_norm_kernel<OT, HT, TPR, 1, kMost><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  } else {
-    constexpr int q = kMost / 4;
-    if (nc <= q) block_norm_kernel<OT, HT, TPR, VEC, q><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else if (nc <= 2 * q) block_norm_kernel<OT, HT, TPR, VEC, 2 * q><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else if (nc <= 3 * q) block_norm_kernel<OT, HT, TPR, VEC, 3 * q><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else block_norm_kernel<OT, HT, TPR, VEC, kMost><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  }
+  constexpr int q = kMost / 4;
+  if (nc <= q) block_norm_kernel<OT, HT, TPR, VEC, q><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else if (nc <= 2 * q) block_norm_kernel<OT, HT, TPR, VEC, 2 * q><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else if (nc <= 3 * q) block_norm_kernel<OT, HT, TPR, VEC, 3 * q><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else block_norm_kernel<OT, HT, TPR, VEC, kMost><<<(unsigned)grid, kThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -361,17 +464,54 @@ cudaError_t norm_types(const BlockNormArgs& a, cudaStream_t st) {
   constexpr int VEC = 16 / (sizeof(OT) > sizeof(HT) ? sizeof(OT) : sizeof(HT));
   const bool vec = a.dim % VEC == 0 && aligned16(a.o, a.ldo, sizeof(OT)) && aligned16(a.h, a.ldh, sizeof(HT)) &&
                    aligned16(a.h_out, a.ldho, sizeof(HT)) && (!a.y || aligned16(a.y, a.ldy, sizeof(OT)));
-  if (a.dim <= 1024) return vec ? norm_chunks<OT, HT, 32, VEC>(a, st) : norm_chunks<OT, HT, 32, 1>(a, st);
-  if (a.dim <= 4096) return vec ? norm_chunks<OT, HT, 128, VEC>(a, st) : norm_chunks<OT, HT, 128, 1>(a, st);
-  return vec ? norm_chunks<OT, HT, 512, VEC>(a, st) : norm_chunks<OT, HT, 512, 1>(a, st);
+  if (vec) {
+    if (a.dim <= 1024) return norm_chunks<OT, HT, 32, VEC>(a, st);
+    if (a.dim <= 4096) return norm_chunks<OT, HT, 128, VEC>(a, st);
+    return norm_chunks<OT, HT, 512, VEC>(a, st);
+  }
+  if (a.dim <= 512) return norm_chunks<OT, HT, 32, 1>(a, st);
+  if (a.dim <= 2048) return norm_chunks<OT, HT, 128, 1>(a, st);
+  return norm_chunks<OT, HT, 512, 1>(a, st);
 }
 
+template <class XT, class YT, class WT, int RU>
+cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units, bool large_too,
+                        const LowRankArgs& a, cudaStream_t st) {
+  const int smem = small_smem_floats(bank.max_rank) * 4;
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  // the largest clusters whose CTAs are all on the device at once (three per SM; two at ranks above 32): 64 units of
+  // rank 16 take 20.5 us on clusters of eight, in two waves, and FOUR us on clusters of four
+  const int room = 132 * (RU <= 4 ? 3 : 2);
+  const int ctas = n_units * 8 <= room ? 8 : n_units * 4 <= room ? 4 : 2;
+  const int clusters = n_units < 2048 ? n_units : 2048;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(clusters * ctas));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, lowrank_small_kernel<XT, YT, WT, RU>, bank, plan, large_too ? 1 : 0, a,
+                            aligned16(a.x, a.ldx, sizeof(XT)) ? 1 : 0);
+}
 template <class XT, class YT>
-cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles, const LowRankArgs& a,
-                        cudaStream_t st) {
-  const int clusters = n_tiles < 4096 ? n_tiles : 4096;
-  lowrank_small_kernel<XT, YT><<<clusters * kSmallCtas, kSmallThreads, 0, st>>>(bank, plan, a);
-  return cudaGetLastError();
+cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units, bool large_too,
+                        const LowRankArgs& a, cudaStream_t st) {
+  auto pick = [&](auto w) {
+    using WT = decltype(w);
+    if (bank.max_rank <= 16) return small_ranks<XT, YT, WT, 2>(bank, plan, n_units, large_too, a, st);
+    if (bank.max_rank <= 32) return small_ranks<XT, YT, WT, 4>(bank, plan, n_units, large_too, a, st);
+    return small_ranks<XT, YT, WT, 16>(bank, plan, n_units, large_too, a, st);
+  };
+  return bank.wtype == kDtF32 ? pick(float()) : pick(uint16_t());
 }
 
 }  // namespace
@@ -385,18 +525,18 @@ cudaError_t launch_adapter_plan(const int32_t* pos, const int32_t* row0, const i
   return cudaGetLastError();
 }
 
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
-                                 const LowRankArgs& a, cudaStream_t st) {
-  if (n_tiles <= 0) return cudaSuccess;
-  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, n_tiles, a, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF16)
-    return small_types<__half, __half>(bank, plan, n_tiles, a, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF32)
-    return small_types<__half, float>(bank, plan, n_tiles, a, st);
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_small, int n_large,
+                                 bool large_too, const LowRankArgs& a, cudaStream_t st) {
+  const int64_t units = (int64_t)n_small + (large_too ? (int64_t)n_large * (kAdapterTileRows / kSmallRows) : 0);
+  if (units <= 0) return cudaSuccess;
+  const int n = units < 0x7fffffff ? (int)units : 0x7fffffff;
+  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, n, large_too, a, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF16) return small_types<__half, __half>(bank, plan, n, large_too, a, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF32) return small_types<__half, float>(bank, plan, n, large_too, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtBF16)
-    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, n_tiles, a, st);
+    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, n, large_too, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtF32)
-    return small_types<__nv_bfloat16, float>(bank, plan, n_tiles, a, st);
+    return small_types<__nv_bfloat16, float>(bank, plan, n, large_too, a, st);
   return cudaErrorInvalidValue;
 }
 

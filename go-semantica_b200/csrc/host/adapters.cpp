@@ -6,6 +6,7 @@
 #include "adapters.h"
 
 #include <array>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -13,6 +14,9 @@
 namespace sem {
 
 namespace {
+
+std::atomic<int> g_lowrank_path{SEM_LOWRANK_PATH_AUTO};
+int get_lowrank_path() { return g_lowrank_path.load(std::memory_order_relaxed); }
 
 bool valid_dtype(int32_t t) { return t == SEM_DTYPE_F32 || t == SEM_DTYPE_F16 || t == SEM_DTYPE_BF16; }
 size_t dtype_size(int32_t t) { return t == SEM_DTYPE_F32 ? 4 : 2; }
@@ -42,7 +46,7 @@ int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapte
   p->max_seqs = max_seqs;
   const int64_t large = adapter_plan_max_large(max_rows, max_seqs);
   // one upload: counts, sequences (pos, row0, seq, adapter), tiles
-  p->up_bytes = 16 + (size_t)round_up((size_t)4 * max_seqs + 4, 4) * 4 + ((size_t)large + max_seqs) * sizeof(AdapterTile);
+  p->up_bytes = 16 + (size_t)round_up((size_t)4 * max_seqs + 4, 4) * 4 + ((size_t)large + max_seqs + 1) * sizeof(AdapterTile);
   cudaError_t e = p->up.ensure(p->up_bytes);
   if (e == cudaSuccess) e = p->maps.ensure((size_t)3 * (max_rows > 0 ? max_rows : 1) * 4);
   if (e == cudaSuccess) e = p->staging.ensure(p->up_bytes);
@@ -62,7 +66,7 @@ AdapterPlanDev plan_device(const sem_adapter_plan* p) {
   const int32_t* maps = p->maps.as<int32_t>();
   return AdapterPlanDev{reinterpret_cast<const int32_t*>(up), tiles,
                         tiles + adapter_plan_max_large(p->max_rows, p->max_seqs), maps, maps + p->max_rows,
-                        maps + 2 * p->max_rows, p->max_rows};
+                        maps + 2 * p->max_rows, p->max_rows, p->max_seqs};
 }
 
 int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapters, int32_t n_seqs, cudaStream_t st) {
@@ -221,15 +225,26 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, const LowRankArgs& ar
 
 }  // namespace
 
+// Up to this many multiply-adds a call runs on the CUDA cores as a whole: the
+// tensor-core kernel's pipeline takes longer to fill than they take. Measured
+// (CUDA cores / tensor cores, 768 x 768, rank 16): INT8 codes 12.6 M 8.3 / 12.0
+// us, 25 M 12.0 / 13.4, 50 M 18.7 / 14.5; float32 rows, whose conversion the
+// tensor cores wait for, 25 M 11.3 / 20.7; 517 x 1001, 168 M 48.8 / 49.9.
+constexpr int64_t kLowRankSmallWork = 28000000, kLowRankSmallWorkF32 = 80000000;
+
 // Both tile lists of the plan. A captured launch may be replayed with a plan
 // set to another batch, so a capture records a launch for each list.
 int lowrank_enqueue(const LowRankBank& bank, const sem_adapter_plan* plan, const LowRankArgs& args, bool captured,
                     uint32_t* err, cudaStream_t st) {
   const AdapterPlanDev dev = plan_device(plan);
-  if (plan->n_large > 0 || captured)
+  const int64_t work = (int64_t)plan->rows * bank.max_rank * (bank.k_in + bank.n_out);
+  const int path = get_lowrank_path();
+  const bool cuda_cores = path == SEM_LOWRANK_PATH_CUDA_CORES || (path == SEM_LOWRANK_PATH_AUTO && work <= (args.xtype == kDtF32 ? kLowRankSmallWorkF32 : kLowRankSmallWork));
+  if (!cuda_cores && (plan->n_large > 0 || captured))
     SEM_CUDA(launch_lowrank_tc(bank, dev, plan->n_large > 0 ? plan->n_large : 1, args, err, st));
-  if (plan->n_small > 0 || captured)
-    SEM_CUDA(launch_lowrank_small(bank, dev, plan->n_small > 0 ? plan->n_small : 1, args, st));
+  if (plan->n_small > 0 || (cuda_cores && plan->n_large > 0) || captured)
+    SEM_CUDA(launch_lowrank_small(bank, dev, plan->n_small > 0 || plan->n_large > 0 ? plan->n_small : 1,
+                                  plan->n_large, cuda_cores, args, st));
   return SEM_OK;
 }
 
@@ -451,6 +466,13 @@ int sem_lowrank_apply_int8(sem_lowrank* w, sem_adapter_plan* plan, const void* d
                            void* stream) {
   return sem::guarded([&]() -> int {
     return sem::lowrank_apply_int8(w, plan, d_codes, d_absmax, n_absmax, d_base, ld_base, d_y, ldy, stream);
+  });
+}
+
+int sem_lowrank_path(int32_t mode) {
+  return sem::guarded([&]() -> int {
+    if (mode < SEM_LOWRANK_PATH_AUTO || mode > SEM_LOWRANK_PATH_TENSOR) return -1;
+    return sem::g_lowrank_path.exchange(mode);
   });
 }
 

@@ -272,6 +272,7 @@ struct AdapterPlanDev {
   const int32_t* pos_seq;      // [rows] and its sequence
   const int32_t* row_adapter;  // [rows]
   int64_t max_rows;            // the plan's capacity
+  int32_t max_seqs;            // small has room for max_seqs + 1 tiles
 };
 // pos_row, pos_seq and row_adapter from the sorted sequences: sequence i of
 // the order holds positions [pos[i], pos[i + 1]) and rows from row0[i] on.
@@ -314,10 +315,10 @@ struct LowRankArgs {
   const uint32_t* absmax;
   int32_t per_seq;
 };
-// The plan's small tiles on CUDA cores (adapters.cu).
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
-                                 const LowRankArgs& args, cudaStream_t stream);
-
+// The plan's small tiles, and with large_too its large ones, on CUDA cores
+// (adapters.cu).
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_small, int n_large,
+                                 bool large_too, const LowRankArgs& args, cudaStream_t stream);
 // The large tiles on the tensor cores (lowrank_tc.cu). `err` (nullable)
 // receives error bits if a pipeline wait times out.
 cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,

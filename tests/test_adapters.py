@@ -151,6 +151,14 @@ def test_block_norm_refusals(dim, eps, n, want):
         _lib.check(_lib.load().sem_block_norm_create(None, dim, eps, None, None, n, None, None, C.byref(h)))
 
 
+def test_lowrank_path_switch():
+    import _lib
+    lib = _lib.load()
+    assert lib.sem_lowrank_path(2) == 0
+    assert lib.sem_lowrank_path(3) == -1 and lib.sem_lowrank_path(-1) == -1
+    assert lib.sem_lowrank_path(0) == 2
+
+
 def test_calls_without_handles():
     import _lib
     lib = _lib.load()
@@ -204,6 +212,16 @@ def _torch(name):
 def _host(w):
     import torch
     return (w.view(torch.int16) if w.dtype == torch.bfloat16 else w).cpu().numpy()
+
+
+@pytest.fixture(params=["auto", "cuda_cores", "tensor"])
+def path(request):
+    """Each kernel for the larger tiles (sem_lowrank_path): small test batches would all take the CUDA cores."""
+    import _lib
+    lib = _lib.load()
+    prev = lib.sem_lowrank_path(["auto", "cuda_cores", "tensor"].index(request.param))
+    yield request.param
+    lib.sem_lowrank_path(prev)
 
 
 class LowRankCase:
@@ -313,7 +331,7 @@ TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf1
 @pytest.mark.parametrize("x,y", TYPES)
 @pytest.mark.parametrize("w", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("shape", range(len(SHAPES)))
-def test_lowrank_types(ctx, shape, x, y, w):
+def test_lowrank_types(ctx, path, shape, x, y, w):
     c = LowRankCase(ctx, *SHAPES[shape], k=96, n=160, x=x, y=y, w=w, seed=shape)
     c.run(ctx)
     c.close()
@@ -323,7 +341,7 @@ def test_lowrank_types(ctx, shape, x, y, w):
 @pytest.mark.parametrize("k,n", [(1, 1), (7, 3), (31, 129), (32, 128), (33, 127), (257, 64), (517, 1001), (768, 768),
                                  (1152, 256)])
 @pytest.mark.parametrize("x", ["f32", "bf16"])
-def test_lowrank_sizes(ctx, k, n, x):
+def test_lowrank_sizes(ctx, path, k, n, x):
     c = LowRankCase(ctx, [1, 40, 130, 2, 260], [0, 1, 2, -1, 1], [4, 19, 128], k, n, x=x, w="bf16", seed=k)
     c.run(ctx)
     c.close()
@@ -333,7 +351,7 @@ def test_lowrank_sizes(ctx, k, n, x):
 @pytest.mark.parametrize("pads", [(0, 0, 0), (1, 3, 5), (8, 8, 8), (4, 0, 12)])
 @pytest.mark.parametrize("base", ["own", "none", "y"])
 @pytest.mark.parametrize("x,y", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
-def test_lowrank_strides_and_base(ctx, pads, base, x, y):
+def test_lowrank_strides_and_base(ctx, path, pads, base, x, y):
     # rank 0 and no adapter: the row is the base (or zeros) whatever the kernel
     c = LowRankCase(ctx, [3, 60, 140, 20, 7], [0, 1, 2, 3, -1], [8, 0, 24, 40], 72, 136, x=x, y=y, w="f16", pads=pads)
     c.run(ctx, base)
@@ -343,7 +361,7 @@ def test_lowrank_strides_and_base(ctx, pads, base, x, y):
 @pytest.mark.gpu
 @pytest.mark.parametrize("codes", [1, 2])
 @pytest.mark.parametrize("w", ["f16", "f32"])
-def test_lowrank_int8_codes(ctx, codes, w):
+def test_lowrank_int8_codes(ctx, path, codes, w):
     c = LowRankCase(ctx, [64, 64, 5, 300, 64], [0, 1, 0, 2, -1], [16, 4, 32], 768, 256, x="f16", y="f32", w=w,
                     codes=codes)
     c.run(ctx)
@@ -354,7 +372,7 @@ def test_lowrank_int8_codes(ctx, codes, w):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [17, 23, 33, 64])
 @pytest.mark.parametrize("k,n,x", [(768, 256, "bf16"), (32, 40, "f32")])
-def test_lowrank_many_short_tiles(ctx, rows, k, n, x):
+def test_lowrank_many_short_tiles(ctx, path, rows, k, n, x):
     # more tiles than SMs, each its own adapter's, most of them shorter than a full one; then a few full ones
     count = 700
     c = LowRankCase(ctx, [rows] * count + [200], [i % 40 if i % 7 else -1 for i in range(count)] + [40],
@@ -381,7 +399,7 @@ def test_lowrank_empty_batch_writes_nothing(ctx):
 
 
 @pytest.mark.gpu
-def test_lowrank_non_finite_rows_stay_their_own(ctx):
+def test_lowrank_non_finite_rows_stay_their_own(ctx, path):
     # infinities and NaN in some rows of x: those rows are the formula's, every other row is finite and right
     import torch
     c = LowRankCase(ctx, [200, 10], [0, 1], [16, 8], 64, 64, w="f16")
@@ -403,7 +421,7 @@ def test_lowrank_non_finite_rows_stay_their_own(ctx):
 
 
 @pytest.mark.gpu
-def test_lowrank_large_values_and_wide_range(ctx):
+def test_lowrank_large_values_and_wide_range(ctx, path):
     # rows of very different magnitude: float32's whole range of exponents through the split operands
     import torch
     c = LowRankCase(ctx, [150, 6], [0, 1], [16, 8], 64, 96, w="f32", pads=(0, 0, 0))
@@ -417,7 +435,7 @@ def test_lowrank_large_values_and_wide_range(ctx):
 
 
 @pytest.mark.gpu
-def test_lowrank_repeats_bit_for_bit_and_alone(ctx):
+def test_lowrank_repeats_bit_for_bit_and_alone(ctx, path):
     # the same rows give the same bits again, and a sequence's rows do not depend on the batch around it
     import torch
     lengths, use, ranks = [300, 20, 7, 150], [0, 1, 2, 1], [16, 24, 8]
@@ -433,7 +451,7 @@ def test_lowrank_repeats_bit_for_bit_and_alone(ctx):
 
 
 @pytest.mark.gpu
-def test_lowrank_streams_and_graph(ctx):
+def test_lowrank_streams_and_graph(ctx, path):
     # two calls at once on two streams with one bank and one plan, then a captured call replayed: first as it was
     # captured, then with other inputs, then with the plan set to another batch (both tile lists change)
     import torch
