@@ -35,6 +35,11 @@ class TensorView(C.Structure):
                 ("data", C.c_void_p), ("nbytes", C.c_uint64)]
 
 
+class AdapterView(C.Structure):
+    """sem_adapter_view: one adapter of a model."""
+    _fields_ = [("tensors", C.POINTER(TensorView)), ("n_tensors", C.c_int32), ("alpha", C.c_float)]
+
+
 class FaithfulConfig(C.Structure):
     """sem_faithful_config: the model-faithful mode (no reference counterpart)."""
     _fields_ = [("sliding_window", C.c_int32), ("swa_pattern", C.c_int32), ("rope_base_swa", C.c_float),
@@ -96,6 +101,10 @@ _SIGNATURES = {
     "sem_block_norm_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
                                      C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                      C.c_void_p]),
+    "sem_model_adapters_create": (C.c_int, [C.c_void_p, C.POINTER(AdapterView), C.c_int32, C.POINTER(C.c_void_p)]),
+    "sem_model_adapters_free": (C.c_int, [C.c_void_p]),
+    "sem_embed_adapted": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                    C.c_void_p]),
     "sem_index_build": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,
                                   C.POINTER(C.c_void_p)]),
     "sem_index_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,

@@ -439,6 +439,29 @@ __global__ void __launch_bounds__(TPR > kNormThreads ? TPR : kNormThreads) block
   }
 }
 
+// A warp per row: gate and up read once, h written once, bound by HBM.
+__global__ void __launch_bounds__(128) gelu_up_kernel(const float* __restrict__ gu, int64_t rows, int F,
+                                                      const int32_t* __restrict__ row_seq, float* __restrict__ h,
+                                                      uint32_t* __restrict__ absmax) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float* g = gu + row * 2 * F;
+  float top = 0.0f;
+  for (int c = (threadIdx.x & 31) * 4; c < F; c += 128) {  // F is a multiple of 128
+    float a[4], b[4];
+    load_vec<4>(g + c, a);
+    load_vec<4>(g + F + c, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __fmul_rn(gelu_quick_ref(a[i]), b[i]);
+      top = fmaxf(top, fabsf(a[i]));
+    }
+    store_vec<4>(h + row * F + c, a);
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) atomicMax(absmax + row_seq[row], __float_as_uint(top));
+}
+
 template <class OT, class HT, int TPR, int VEC>
 cudaError_t norm_chunks(const BlockNormArgs& a, cudaStream_t st) {
   constexpr int kThreads = TPR > kNormThreads ? TPR : kNormThreads;
@@ -538,6 +561,14 @@ cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& 
   if (a.xtype == kDtBF16 && a.ytype == kDtF32)
     return small_types<__nv_bfloat16, float>(bank, plan, n, large_too, a, st);
   return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_gelu_up(const float* gu, int64_t rows, int F, const int32_t* row_seq, float* h, uint32_t* absmax,
+                           cudaStream_t st) {
+  if (rows <= 0) return cudaSuccess;
+  if (F % 128 || (rows + 3) / 4 > 0x7fffffff) return cudaErrorInvalidValue;
+  gelu_up_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(gu, rows, F, row_seq, h, absmax);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_block_norm(const BlockNormArgs& a, cudaStream_t st) {

@@ -35,6 +35,8 @@ int capturing(cudaStream_t st, bool* out) {
   return SEM_OK;
 }
 
+}  // namespace
+
 int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapter_plan** out) {
   if (max_rows < 0 || max_rows > 0x7fffffff || max_seqs < 0 || max_seqs == 0x7fffffff)
     return set_error(SEM_EINVAL, "adapter plan: at most 2147483647 rows and 2147483646 sequences");
@@ -57,8 +59,6 @@ int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapte
   *out = p.release();
   return SEM_OK;
 }
-
-}  // namespace
 
 AdapterPlanDev plan_device(const sem_adapter_plan* p) {
   const uint8_t* up = p->up.as<uint8_t>();
@@ -314,6 +314,8 @@ int lowrank_check(sem_lowrank* w) {
   return SEM_OK;
 }
 
+}  // namespace
+
 int block_norm_create(sem_context* ctx, int32_t dim, float eps, const float* post_w, const float* pre_w,
                       int32_t n_adapters, const float* gates, const float* scales, sem_block_norm** out) {
   if (dim <= 0 || dim > kBlockNormMaxDim)
@@ -351,6 +353,24 @@ int block_norm_create(sem_context* ctx, int32_t dim, float eps, const float* pos
   return SEM_OK;
 }
 
+BlockNormArgs block_norm_args(const sem_block_norm* b, const sem_adapter_plan* plan, int64_t rows) {
+  BlockNormArgs a{};
+  a.ldo = a.ldh = a.ldho = a.ldy = b->dim;
+  a.dtype = a.htype = kDtF32;
+  a.rows = rows;
+  a.dim = b->dim;
+  a.eps = b->eps;
+  a.post = b->post;
+  a.pre = b->pre;
+  a.gates = b->gates;
+  a.scales = b->scales;
+  a.n_adapters = b->n_adapters;
+  a.row_adapter = plan ? plan_device(plan).row_adapter : nullptr;
+  return a;
+}
+
+namespace {
+
 int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, const void* d_o, int64_t ldo,
                    int32_t dtype, const void* d_h, int64_t ldh, int32_t h_dtype, void* d_h_out, int64_t ldho,
                    void* d_y, int64_t ldy, void* stream) {
@@ -369,7 +389,6 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
     return set_error(SEM_EINVAL, "block norm: a pointer is not aligned to its element type");
   if ((d_h_out == d_h && ldho != ldh) || (b->pre && d_y == d_o && ldy != ldo))
     return set_error(SEM_EINVAL, "block norm: one buffer with two row strides");
-  const int32_t* row_adapter = nullptr;
   DeviceGuard dg(b->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : b->ctx->stream;
   if (plan) {
@@ -380,9 +399,8 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
     if ((b->gates || b->scales) && plan->max_adapter >= b->n_adapters)
       return set_error(SEM_EINVAL, "block norm: the plan uses adapter %d, there are %d", plan->max_adapter,
                        b->n_adapters);
-    row_adapter = plan_device(plan).row_adapter;
   }
-  BlockNormArgs a{};
+  BlockNormArgs a = block_norm_args(b, plan, rows);
   a.o = d_o;
   a.h = d_h;
   a.h_out = d_h_out;
@@ -393,15 +411,6 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
   a.ldy = ldy;
   a.dtype = dtype;
   a.htype = h_dtype;
-  a.rows = rows;
-  a.dim = b->dim;
-  a.eps = b->eps;
-  a.post = b->post;
-  a.pre = b->pre;
-  a.gates = b->gates;
-  a.scales = b->scales;
-  a.n_adapters = b->n_adapters;
-  a.row_adapter = row_adapter;
   SEM_CUDA(launch_block_norm(a, st));
   return SEM_OK;
 }

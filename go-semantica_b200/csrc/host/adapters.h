@@ -36,11 +36,17 @@ namespace sem {
 
 constexpr int32_t kLowRankMaxDim = 65536;
 
+int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapter_plan** out);
 int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapters, int32_t n_seqs, cudaStream_t st);
 AdapterPlanDev plan_device(const sem_adapter_plan* p);
 int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adapters, const int32_t* ranks,
                    const float* scales, const void* const* a, const void* const* b, int32_t dtype, sem_lowrank** out);
 int lowrank_enqueue(const LowRankBank& bank, const sem_adapter_plan* plan, const LowRankArgs& args, bool captured,
                     uint32_t* err, cudaStream_t st);
+
+// The arguments of a block norm over packed rows with the plan's adapters.
+BlockNormArgs block_norm_args(const sem_block_norm* b, const sem_adapter_plan* plan, int64_t rows);
+int block_norm_create(sem_context* ctx, int32_t dim, float eps, const float* post_w, const float* pre_w,
+                      int32_t n_adapters, const float* gates, const float* scales, sem_block_norm** out);
 
 }  // namespace sem

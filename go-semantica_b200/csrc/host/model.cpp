@@ -8,6 +8,7 @@
 #include <string>
 #include <vector>
 
+#include "adapters.h"
 #include "gguf.h"
 #include "internal.h"
 
@@ -97,6 +98,21 @@ struct sem_model {
   sem::Q8Proj dense2{}, dense3{};
   int32_t dense_mid = 0;      // dense_2 output width
   sem::DevBuf head_y1, head_codes, head_absmax;
+  // sem_embed_adapted: the batch's row -> adapter plan, gate and up before GELU
+  std::unique_ptr<sem_adapter_plan> plan;
+  sem::DevBuf gate_up;
+};
+
+// Adapters of a model: per layer a bank for each projection that any of them
+// touches, and block norms where any of them has a gate or residual scale.
+struct sem_model_adapters {
+  sem_model* model = nullptr;
+  int32_t n = 0;
+  struct Layer {
+    std::unique_ptr<sem_lowrank> proj[7];  // kAdapterProjs' order
+    std::unique_ptr<sem_block_norm> attn, ffn;
+  };
+  std::vector<Layer> layers;
 };
 
 
@@ -532,11 +548,12 @@ int upload_meta(sem_model* m, const int32_t* offsets, int B, const int32_t* dims
 }
 
 // Stage ids for the optional per-launch timing (sem_model_profile).
+// (kStAdapters: the low-rank products and the block norms of sem_embed_adapted)
 enum Stage { kStEmbed, kStRowStats, kStQuant, kStGemmQKV, kStQKNormRope, kStAttention, kStGemmO, kStResidual,
-             kStGemmGateUp, kStGemmDown, kStPool, kStAttnShort, kStages };
+             kStGemmGateUp, kStGemmDown, kStPool, kStAttnShort, kStAdapters, kStages };
 const char* const kStageNames[kStages] = {"embed", "row_stats", "quantize", "gemm_q8_qkv", "qk_norm_rope", "attention",
                                           "gemm_q8_o", "residual_norm", "gemm_q8_gate_up", "gemm_q8_down", "pool_l2",
-                                          "attention_short"};
+                                          "attention_short", "adapters"};
 
 }  // namespace
 
@@ -553,8 +570,13 @@ namespace {
     if (m->prof) prof_mark(m, (stage), st, true);                                               \
   } while (0)
 
+enum AdapterProj { kAdQ, kAdK, kAdV, kAdO, kAdGate, kAdUp, kAdDown, kAdProjs };
+const char* const kAdapterProjs[kAdProjs] = {"attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down"};
+
 // The whole forward on `st`: ids already on the device in m->ids (or d_ids).
-int run_forward(sem_model* m, const int32_t* d_ids, const MetaPtrs& mp, float* d_out, cudaStream_t st) {
+// With `ad`, the sequences' adapters by m->plan (sem_embed_adapted).
+int run_forward(sem_model* m, const int32_t* d_ids, const MetaPtrs& mp, float* d_out, cudaStream_t st,
+                const sem_model_adapters* ad = nullptr) {
   const sem_model_config& c = m->cfg;
   const int H = c.embed_dim, F = c.interm_dim, L = c.num_layers, nh = c.num_heads, hd = c.head_dim;
   const int qkvN = nh * hd + 2 * hd;
@@ -598,6 +620,33 @@ int run_forward(sem_model* m, const int32_t* d_ids, const MetaPtrs& mp, float* d
     }
     return e;
   };
+  // y += the low-rank product of a projection's codes with every sequence's adapter (rows ld apart)
+  auto low_rank = [&](int l, int proj, const uint32_t* a_absmax, float* y, int64_t ld) -> int {
+    const sem_lowrank* w = ad ? ad->layers[l].proj[proj].get() : nullptr;
+    if (!w) return SEM_OK;
+    const LowRankArgs args{codes, y, y, w->bank.k_in, ld, ld, kDtF16, kDtF32, a_absmax, 1};
+    if (m->prof) prof_mark(m, kStAdapters, st, false);
+    const int rc = lowrank_enqueue(w->bank, m->plan.get(), args, false, err, st);
+    if (m->prof) prof_mark(m, kStAdapters, st, true);
+    return rc;
+  };
+  // residual and next norm with gates and residual scales: hid, and the norm's codes (or inv_rms at the end)
+  auto gated = [&](const sem_block_norm* b, const float* o, float* normed, uint32_t* next_absmax) -> int {
+    BlockNormArgs a = block_norm_args(b, m->plan.get(), T);
+    a.o = o;
+    a.h = a.h_out = hid;
+    a.y = normed;
+    a.row_seq = sm.row_seq;
+    a.absmax = next_absmax;
+    if (!next_absmax) a.pre = nullptr;
+    SEM_LAUNCH(kStAdapters, launch_block_norm(a, st));
+    if (next_absmax) {
+      SEM_LAUNCH(kStQuant, launch_quantize(normed, nullptr, nullptr, H, sm, next_absmax, codes, st));
+    } else {
+      SEM_LAUNCH(kStRowStats, launch_row_stats(hid, b->pre, H, c.norm_eps, sm, inv, nullptr, st));
+    }
+    return SEM_OK;
+  };
   SEM_LAUNCH(kStEmbed, cudaMemsetAsync(amax, 0, (size_t)(4 * L + 1) * B * 4, st));
   SEM_LAUNCH(kStEmbed, launch_embed(d_ids, m->emb, m->emb_s, c.vocab_size, H, hid, (int)T, m->errflag.as<uint32_t>(), st));
   SEM_LAUNCH(kStRowStats, launch_row_stats(hid, m->layers[0].attn_norm, H, c.norm_eps, sm, inv, slot(0, 0), st));
@@ -617,9 +666,15 @@ int run_forward(sem_model* m, const int32_t* d_ids, const MetaPtrs& mp, float* d
     // attention block (model_int8.go:191-210)
     // the long rows' V columns go straight to the attention's hi / lo planes
     // when the split-plane kernel projects them (v_planes: it did)
+    // (not where an adapter adds to V)
     bool v_planes = false;
+    const sem_model_adapters::Layer* al = ad ? &ad->layers[l] : nullptr;
     SEM_LAUNCH(kStGemmQKV, q8(w.qkv, qkvN, H, slot(l, 0), big, qkvN, kEpiStore, nullptr,
-                              VPlanes{vh, T, nh * hd + hd, &v_planes}));
+                              al && al->proj[kAdV] ? VPlanes{} : VPlanes{vh, T, nh * hd + hd, &v_planes}));
+    int rc;
+    if ((rc = low_rank(l, kAdQ, slot(l, 0), big, qkvN))) return rc;
+    if ((rc = low_rank(l, kAdK, slot(l, 0), big + nh * hd, qkvN))) return rc;
+    if ((rc = low_rank(l, kAdV, slot(l, 0), big + nh * hd + hd, qkvN))) return rc;
     SEM_LAUNCH(kStQKNormRope, launch_qk_norm_rope(big, w.q_norm, w.k_norm, sliding ? swa_cos : m->rope_cos,
                                                   sliding ? swa_sin : m->rope_sin, c.norm_eps, nh, sm, qh, ql, kh, kl,
                                                   vh, vl, exact_short ? mp.T_long : T,
@@ -638,14 +693,32 @@ int run_forward(sem_model* m, const int32_t* d_ids, const MetaPtrs& mp, float* d
     }
     SEM_LAUNCH(kStQuant, launch_quantize(att, nullptr, nullptr, H, sm, slot(l, 1), codes, st));
     SEM_LAUNCH(kStGemmO, q8(w.o, H, H, slot(l, 1), big, H, kEpiStore, nullptr));
-    SEM_LAUNCH(kStResidual, launch_residual_norm(big, w.post_attn, hid, w.ffn_norm, H, c.norm_eps, sm, inv, slot(l, 2),
-                                                 codes, st));
+    if ((rc = low_rank(l, kAdO, slot(l, 1), big, H))) return rc;
+    if (al && al->attn) {
+      if ((rc = gated(al->attn.get(), big, att, slot(l, 2)))) return rc;
+    } else {
+      SEM_LAUNCH(kStResidual, launch_residual_norm(big, w.post_attn, hid, w.ffn_norm, H, c.norm_eps, sm, inv, slot(l, 2),
+                                                   codes, st));
+    }
     // MLP block (model_int8.go:213-232)
-    SEM_LAUNCH(kStGemmGateUp, q8(w.gu, 2 * F, H, slot(l, 2), big, F, kEpiGeluUp, slot(l, 3)));
+    if (al && (al->proj[kAdGate] || al->proj[kAdUp])) {
+      float* gu = m->gate_up.as<float>();
+      SEM_LAUNCH(kStGemmGateUp, q8(w.gu, 2 * F, H, slot(l, 2), gu, 2 * F, kEpiStore, nullptr));
+      if ((rc = low_rank(l, kAdGate, slot(l, 2), gu, 2 * F))) return rc;
+      if ((rc = low_rank(l, kAdUp, slot(l, 2), gu + F, 2 * F))) return rc;
+      SEM_LAUNCH(kStAdapters, launch_gelu_up(gu, T, F, sm.row_seq, big, slot(l, 3), st));
+    } else {
+      SEM_LAUNCH(kStGemmGateUp, q8(w.gu, 2 * F, H, slot(l, 2), big, F, kEpiGeluUp, slot(l, 3)));
+    }
     SEM_LAUNCH(kStQuant, launch_quantize(big, nullptr, nullptr, F, sm, slot(l, 3), codes, st));
     SEM_LAUNCH(kStGemmDown, q8(w.down, H, F, slot(l, 3), att, H, kEpiStore, nullptr));
+    if ((rc = low_rank(l, kAdDown, slot(l, 3), att, H))) return rc;
     const bool last = l + 1 == L;
     const float* next_w = last ? m->out_norm : m->layers[l + 1].attn_norm;
+    if (al && al->ffn) {
+      if ((rc = gated(al->ffn.get(), att, big, last ? nullptr : slot(l + 1, 0)))) return rc;
+      continue;
+    }
     SEM_LAUNCH(kStResidual, launch_residual_norm(att, w.post_ffw, hid, next_w ? next_w : w.ffn_norm, H, c.norm_eps, sm, inv,
                                                  last ? nullptr : slot(l + 1, 0), last ? nullptr : codes, st));
   }
@@ -759,6 +832,33 @@ int forward_maybe_graph(sem_model* m, const MetaPtrs& mp, const int32_t* offsets
   return SEM_OK;
 }
 
+// The plan of a batch for the forward's packed rows: sequences of >=
+// kSplitMinLen tokens first, as upload_meta packs them.
+int adapter_plan_for(sem_model* m, const int32_t* offsets, int B, const int32_t* use) {
+  std::vector<int32_t> packed(1, 0), adapters;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int s = 0; s < B; ++s) {
+      const int32_t len = offsets[s + 1] - offsets[s];
+      if ((len >= kSplitMinLen) != (pass == 0)) continue;
+      packed.push_back(packed.back() + len);
+      adapters.push_back(use[s]);
+    }
+  if (!m->plan || m->plan->max_rows < offsets[B] || m->plan->max_seqs < B) {
+    SEM_CUDA(cudaStreamSynchronize(m->ctx->stream));  // the old plan may still be read
+    sem_adapter_plan* p = nullptr;
+    const int64_t rows = m->plan ? std::max<int64_t>(m->plan->max_rows, offsets[B]) : offsets[B];
+    if (int rc = plan_create(m->ctx, rows, std::max(B, m->plan ? m->plan->max_seqs : 0), &p)) return rc;
+    m->plan.reset(p);
+  }
+  return plan_set(m->plan.get(), packed.data(), adapters.data(), B, m->ctx->stream);
+}
+
+bool adapters_gate_up(const sem_model_adapters* ad) {
+  for (const auto& l : ad->layers)
+    if (l.proj[kAdGate] || l.proj[kAdUp]) return true;
+  return false;
+}
+
 }  // namespace
 
 int validate_embed_request(const sem_model_config& c, const int32_t* ids, const int32_t* offsets, int32_t B,
@@ -785,7 +885,7 @@ int validate_embed_request(const sem_model_config& c, const int32_t* ids, const 
 }
 
 int model_embed(sem_model* m, const int32_t* ids, const int32_t* offsets, int32_t B, const int32_t* dims_in,
-                float* out) {
+                float* out, const sem_model_adapters* ad = nullptr, const int32_t* use = nullptr) {
   if (!m) return set_error(SEM_EINVAL, "null argument");
   std::vector<int32_t> dims;
   int64_t out_floats = 0;
@@ -806,7 +906,14 @@ int model_embed(sem_model* m, const int32_t* ids, const int32_t* offsets, int32_
   } else {
     SEM_CUDA(cudaMemcpyAsync(m->ids.p, ids, (size_t)T * 4, cudaMemcpyHostToDevice, ctx->stream));
   }
-  if ((rc = forward_maybe_graph(m, mp, offsets, dims.data(), ctx->stream))) return rc;
+  if (ad) {
+    if ((rc = adapter_plan_for(m, offsets, B, use))) return rc;
+    if (adapters_gate_up(ad)) SEM_CUDA(m->gate_up.ensure((size_t)T * 2 * m->cfg.interm_dim * 4));
+    rc = run_forward(m, m->ids.as<int32_t>(), mp, m->out.as<float>(), ctx->stream, ad);
+  } else {
+    rc = forward_maybe_graph(m, mp, offsets, dims.data(), ctx->stream);
+  }
+  if (rc) return rc;
   SEM_CUDA(cudaMemcpyAsync(out, m->out.p, (size_t)out_floats * 4, cudaMemcpyDeviceToHost, ctx->stream));
   SEM_CUDA(ctx->pinned.ensure(64));
   uint32_t* flags = ctx->pinned.as<uint32_t>();
@@ -991,6 +1098,174 @@ int model_embed_device(sem_model* m, const int32_t* d_ids, const int32_t* h_offs
     d_ids = m->ids.as<int32_t>();
   }
   return run_forward(m, d_ids, mp, d_out, st);
+}
+
+// ---------------------------------------------------------------------------
+// Adapters of the model (sem_embed_adapted)
+// ---------------------------------------------------------------------------
+int embed_adapted(sem_model* m, sem_model_adapters* ad, const int32_t* ids, const int32_t* offsets, int32_t B,
+                  const int32_t* use, const int32_t* dims, float* out) {
+  if (!m || !ad || (!use && B > 0)) return set_error(SEM_EINVAL, "null argument");
+  if (ad->model != m) return set_error(SEM_EINVAL, "the adapters belong to another model");
+  bool any = false;
+  for (int32_t s = 0; s < B; ++s) {
+    if (use[s] < -1 || use[s] >= ad->n) return set_error(SEM_EINVAL, "adapter %d out of range (-1..%d)", use[s], ad->n - 1);
+    any |= use[s] >= 0;
+  }
+  return any ? model_embed(m, ids, offsets, B, dims, out, ad, use) : model_embed(m, ids, offsets, B, dims, out);
+}
+
+namespace {
+
+constexpr uint32_t kF16 = 1, kBF16 = 30;
+
+float half_bits(uint16_t h) {
+  __half_raw r;
+  r.x = h;
+  return __half2float(__half(r));
+}
+float bf16_bits(uint16_t h) {
+  const uint32_t w = (uint32_t)h << 16;
+  float f;
+  std::memcpy(&f, &w, 4);
+  return f;
+}
+
+// One layer's bank of projection `proj`, or none when no adapter touches it:
+// in the adapters' own type when they all have the same, else in float32.
+int adapter_bank(sem_model* m, const sem_adapter_view* av, int32_t n, int layer, int proj, int32_t k, int32_t n_out,
+                 std::unique_ptr<sem_lowrank>* out) {
+  char na[128], nb[128];
+  snprintf(na, sizeof na, "blk.%d.%s.weight.lora_a", layer, kAdapterProjs[proj]);
+  snprintf(nb, sizeof nb, "blk.%d.%s.weight.lora_b", layer, kAdapterProjs[proj]);
+  std::vector<const sem_tensor_view*> ta(n), tb(n);
+  std::vector<int32_t> ranks(n, 0);
+  std::vector<float> scales(n, 0.0f);
+  uint32_t type = ~0u;
+  bool any = false;
+  for (int32_t i = 0; i < n; ++i) {
+    ta[i] = find_view(av[i].tensors, av[i].n_tensors, na);
+    tb[i] = find_view(av[i].tensors, av[i].n_tensors, nb);
+    if (!ta[i] && !tb[i]) continue;
+    if (!ta[i] || !tb[i]) return set_error(SEM_EFORMAT, "adapter %d: %s without its other half", i, ta[i] ? na : nb);
+    any = true;
+    const sem_tensor_view& a = *ta[i];
+    const sem_tensor_view& b = *tb[i];
+    if (a.n_dims < 2 || b.n_dims < 2 || a.dims[0] != (uint64_t)k || b.dims[1] != (uint64_t)n_out ||
+        a.dims[1] != b.dims[0] || a.dims[1] < 1 || a.dims[1] > (uint64_t)kLowRankMaxRank)
+      return set_error(SEM_EFORMAT, "adapter %d: %s {%llu,%llu} and lora_b {%llu,%llu}, want {%d,rank} and {rank,%d}, rank 1..%d",
+                       i, na, (unsigned long long)a.dims[0], (unsigned long long)(a.n_dims > 1 ? a.dims[1] : 0),
+                       (unsigned long long)b.dims[0], (unsigned long long)(b.n_dims > 1 ? b.dims[1] : 0), k, n_out,
+                       kLowRankMaxRank);
+    ranks[i] = (int32_t)a.dims[1];
+    scales[i] = av[i].alpha == 0.0f ? 1.0f : av[i].alpha / (float)ranks[i];
+    for (const sem_tensor_view* t : {ta[i], tb[i]}) {
+      if (t->dtype != kF32 && t->dtype != kF16 && t->dtype != kBF16)
+        return set_error(SEM_EFORMAT, "adapter %d: %s: type %u, want F32, F16 or BF16", i, t->name, t->dtype);
+      if (!t->data || t->nbytes < t->dims[0] * t->dims[1] * (t->dtype == kF32 ? 4 : 2))
+        return set_error(SEM_EFORMAT, "adapter %d: %s: %llu bytes", i, t->name, (unsigned long long)t->nbytes);
+      type = type == ~0u || type == t->dtype ? t->dtype : kF32;
+    }
+  }
+  if (!any) return SEM_OK;
+  std::vector<std::vector<float>> wide;  // float32 copies where the types differ
+  wide.reserve((size_t)2 * n);
+  auto bytes = [&](const sem_tensor_view* t) -> const void* {
+    if (!t) return nullptr;
+    if (t->dtype == type) return t->data;
+    const size_t count = (size_t)(t->dims[0] * t->dims[1]);
+    wide.emplace_back(count);
+    const uint16_t* h = static_cast<const uint16_t*>(t->data);
+    for (size_t j = 0; j < count; ++j) wide.back()[j] = t->dtype == kF16 ? half_bits(h[j]) : bf16_bits(h[j]);
+    return wide.back().data();
+  };
+  std::vector<const void*> pa(n), pb(n);
+  for (int32_t i = 0; i < n; ++i) {
+    pa[i] = bytes(ta[i]);
+    pb[i] = bytes(tb[i]);
+  }
+  sem_lowrank* w = nullptr;
+  const int32_t dt = type == kF32 ? SEM_DTYPE_F32 : type == kF16 ? SEM_DTYPE_F16 : SEM_DTYPE_BF16;
+  if (int rc = lowrank_create(m->ctx, k, n_out, n, ranks.data(), scales.data(), pa.data(), pb.data(), dt, &w)) return rc;
+  out->reset(w);
+  return SEM_OK;
+}
+
+// The block norm after a layer's attention or MLP, when any adapter has a gate
+// or residual scale there: the model's own norm weights, read back.
+int adapter_norm(sem_model* m, const sem_adapter_view* av, int32_t n, int layer, const char* block, const float* d_post,
+                 const float* d_pre, std::unique_ptr<sem_block_norm>* out) {
+  const int H = m->cfg.embed_dim;
+  char ng[128], ns[128];
+  snprintf(ng, sizeof ng, "blk.%d.%s.gate", layer, block);
+  snprintf(ns, sizeof ns, "blk.%d.%s.scale", layer, block);
+  std::vector<float> gates((size_t)n * H, 1.0f), scales(n, 1.0f);
+  bool any = false;
+  for (int32_t i = 0; i < n; ++i)
+    for (const char* name : {ng, ns}) {
+      const sem_tensor_view* t = find_view(av[i].tensors, av[i].n_tensors, name);
+      if (!t) continue;
+      const size_t want = name == ng ? (size_t)H : 1;
+      if (t->dtype != kF32 || t->n_dims < 1 || t->dims[0] != want || !t->data || t->nbytes < want * 4)
+        return set_error(SEM_EFORMAT, "adapter %d: %s: want %zu F32 values", i, name, want);
+      std::memcpy(name == ng ? &gates[(size_t)i * H] : &scales[i], t->data, want * 4);
+      any = true;
+    }
+  if (!any) return SEM_OK;
+  std::vector<float> post(H), pre(H, 1.0f);
+  if (d_post) SEM_CUDA(cudaMemcpy(post.data(), d_post, (size_t)H * 4, cudaMemcpyDeviceToHost));
+  if (d_pre) SEM_CUDA(cudaMemcpy(pre.data(), d_pre, (size_t)H * 4, cudaMemcpyDeviceToHost));
+  sem_block_norm* b = nullptr;
+  if (int rc = block_norm_create(m->ctx, H, m->cfg.norm_eps, d_post ? post.data() : nullptr, pre.data(), n, gates.data(),
+                                 scales.data(), &b))
+    return rc;
+  out->reset(b);
+  return SEM_OK;
+}
+
+}  // namespace
+
+int adapters_create(sem_model* m, const sem_adapter_view* av, int32_t n, sem_model_adapters** out) {
+  if (n < 0) return set_error(SEM_EINVAL, "adapters: negative count %d", n);
+  if (!m || !out || (n > 0 && !av)) return set_error(SEM_EINVAL, "null argument");
+  const sem_model_config& c = m->cfg;
+  const int H = c.embed_dim, F = c.interm_dim, hd = c.head_dim;
+  const int32_t in[kAdProjs] = {H, H, H, c.num_heads * hd, H, H, F};
+  const int32_t wide[kAdProjs] = {c.num_heads * hd, hd, hd, H, F, F, H};
+  for (int32_t i = 0; i < n; ++i) {  // every tensor is one that the model has a place for
+    if (av[i].n_tensors < 0 || (av[i].n_tensors > 0 && !av[i].tensors)) return set_error(SEM_EINVAL, "null argument");
+    if (!std::isfinite(av[i].alpha)) return set_error(SEM_EINVAL, "adapter %d: alpha must be finite", i);
+    for (int32_t k = 0; k < av[i].n_tensors; ++k) {
+      const char* name = av[i].tensors[k].name ? av[i].tensors[k].name : "";
+      int layer = -1, used = 0;
+      bool known = false;
+      if (sscanf(name, "blk.%d.%n", &layer, &used) == 1 && used > 0 && layer >= 0 && layer < c.num_layers) {
+        const std::string rest = name + used;
+        const bool plain = "blk." + std::to_string(layer) + "." + rest == name;  // no leading zeros or signs
+        for (const char* p : kAdapterProjs)
+          known |= plain && (rest == std::string(p) + ".weight.lora_a" || rest == std::string(p) + ".weight.lora_b");
+        for (const char* b : {"attn_residual", "ffn_residual"})
+          known |= plain && (rest == std::string(b) + ".gate" || rest == std::string(b) + ".scale");
+      }
+      if (!known) return set_error(SEM_EFORMAT, "adapter %d: unknown tensor %s", i, name);
+    }
+  }
+  DeviceGuard dg(m->ctx->device);
+  std::unique_ptr<sem_model_adapters> a(new sem_model_adapters());
+  a->model = m;
+  a->n = n;
+  a->layers.resize(c.num_layers);
+  for (int l = 0; l < c.num_layers; ++l) {
+    auto& L = a->layers[l];
+    for (int p = 0; p < kAdProjs; ++p)
+      if (int rc = adapter_bank(m, av, n, l, p, in[p], wide[p], &L.proj[p])) return rc;
+    const LayerW& w = m->layers[l];
+    const float* next = l + 1 < c.num_layers ? m->layers[l + 1].attn_norm : m->out_norm;
+    if (int rc = adapter_norm(m, av, n, l, "attn_residual", w.post_attn, w.ffn_norm, &L.attn)) return rc;
+    if (int rc = adapter_norm(m, av, n, l, "ffn_residual", w.post_ffw, next, &L.ffn)) return rc;
+  }
+  *out = a.release();
+  return SEM_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -1216,6 +1491,25 @@ int sem_embed(sem_model* m, const int32_t* ids, const int32_t* offsets, int32_t 
   return sem::guarded([&]() -> int {
     return sem::model_embed(m, ids, offsets, n, dims, out);
   });
+}
+
+int sem_model_adapters_create(sem_model* m, const sem_adapter_view* adapters, int32_t n, sem_model_adapters** out) {
+  return sem::guarded([&]() -> int { return sem::adapters_create(m, adapters, n, out); });
+}
+
+int sem_model_adapters_free(sem_model_adapters* a) {
+  return sem::guarded([&]() -> int {
+    if (!a) return SEM_OK;
+    sem::DeviceGuard dg(a->model->ctx->device);
+    cudaStreamSynchronize(a->model->ctx->stream);
+    delete a;
+    return SEM_OK;
+  });
+}
+
+int sem_embed_adapted(sem_model* m, sem_model_adapters* adapters, const int32_t* ids, const int32_t* offsets, int32_t n,
+                      const int32_t* use, const int32_t* dims, float* out) {
+  return sem::guarded([&]() -> int { return sem::embed_adapted(m, adapters, ids, offsets, n, use, dims, out); });
 }
 
 int sem_embed_submit(sem_model* m, const int32_t* ids, const int32_t* offsets, int32_t n, const int32_t* dims,

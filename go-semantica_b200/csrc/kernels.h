@@ -173,6 +173,12 @@ cudaError_t launch_q8_proj(const __half* a_codes, const Q8Proj& w, int M, int N,
 int set_q8_path(int mode);
 int get_q8_path();
 
+// h = gelu_quick(gate) * up for rows of gu [gate F | up F], as the kEpiGeluUp
+// epilogues compute it; absmax[row_seq[row]] receives the atomic max of |h|
+// (adapted projections add to gate and up before it).
+cudaError_t launch_gelu_up(const float* gu, int64_t rows, int F, const int32_t* row_seq, float* h, uint32_t* absmax,
+                           cudaStream_t stream);
+
 // ---- attention (attention.cu) ----
 constexpr int kAttnTileRows = 128;  // query rows per attention tile
 struct AttnTiles {

@@ -65,6 +65,34 @@ class Model:
             o += int(k)
         return res
 
+    # ---- adapters ----
+    def load_adapters(self, adapters) -> "ModelAdapters":
+        """sem_model_adapters_create: a list of (tensors, alpha), tensors as for
+        load_model_from_views with the names and types of sem_adapter_view."""
+        return ModelAdapters(self, adapters)
+
+    def forward_batch_adapted(self, adapters: "ModelAdapters", ids, offsets, use, dims=None) -> list[np.ndarray]:
+        """forward_batch with adapter use[s] (-1: none) for each sequence (sem_embed_adapted)."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        offsets = np.ascontiguousarray(offsets, dtype=np.int32)
+        use = np.ascontiguousarray(use, dtype=np.int32)
+        n = offsets.size - 1
+        if use.size != n:
+            raise ValueError(f"{use.size} adapters for {n} sequences")
+        if dims is None:
+            dims = [self._config.embed_dim] * n
+        elif np.isscalar(dims):
+            dims = [int(dims)] * n
+        d = np.ascontiguousarray(dims, dtype=np.int32)
+        out = np.empty(max(int(d[d > 0].sum()) if n else 0, 1), dtype=np.float32)
+        check(load().sem_embed_adapted(self.handle, adapters.handle, ids.ctypes.data, offsets.ctypes.data, n,
+                                       use.ctypes.data, d.ctypes.data, out.ctypes.data))
+        res, o = [], 0
+        for k in d:
+            res.append(out[o:o + int(k)].copy())
+            o += int(k)
+        return res
+
     # ---- request pipeline ----
     def submit(self, ids, offsets, dims=None) -> tuple:
         """sem_embed_submit: enqueues a request and returns its ticket without
@@ -149,6 +177,34 @@ class Model:
         check(load().sem_model_check(self.handle))
 
 
+class ModelAdapters:
+    """Adapters of one model on its device (sem_model_adapters)."""
+
+    def __init__(self, model: Model, adapters):
+        self.model = model  # outlives its adapters
+        self.handle = None
+        keep, views = [], (_lib.AdapterView * max(len(adapters), 1))()
+        for i, (tensors, alpha) in enumerate(adapters):
+            tv = _tensor_views(tensors, keep)
+            keep.append(tv)
+            views[i].tensors, views[i].n_tensors, views[i].alpha = tv, len(tensors), alpha
+        h = C.c_void_p()
+        check(load().sem_model_adapters_create(model.handle, views, len(adapters), C.byref(h)))
+        self.handle, self.count = h, len(adapters)
+
+    def close(self) -> None:
+        if self.handle:
+            load().sem_model_adapters_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.model.handle:
+                self.close()
+        except Exception:
+            pass
+
+
 class Group:
     """Several devices as one embedding engine (sem_group_*): a model replica
     per device, each request split across them by token count and embedded on
@@ -221,11 +277,9 @@ def load_model(path: str, ctx: Context | None = None) -> Model:
     return Model(ctx, h)
 
 
-def load_model_from_views(ctx: Context, config: ModelConfig, tensors: dict) -> Model:
-    """sem_model_load with tensor views (the path a Go loader takes through cgo).
-    tensors: name -> (dtype, dims tuple, numpy buffer)."""
-    keep = []
-    views = (TensorView * len(tensors))()
+def _tensor_views(tensors: dict, keep: list):
+    """sem_tensor_view array of {name: (dtype, dims, array)}; what it points to is added to `keep`."""
+    views = (TensorView * max(len(tensors), 1))()
     for i, (name, (dtype, dims, buf)) in enumerate(tensors.items()):
         b = np.ascontiguousarray(buf)
         keep.append(b)
@@ -238,6 +292,14 @@ def load_model_from_views(ctx: Context, config: ModelConfig, tensors: dict) -> M
             views[i].dims[k] = dv
         views[i].data = b.ctypes.data
         views[i].nbytes = b.nbytes
+    return views
+
+
+def load_model_from_views(ctx: Context, config: ModelConfig, tensors: dict) -> Model:
+    """sem_model_load with tensor views (the path a Go loader takes through cgo).
+    tensors: name -> (dtype, dims tuple, numpy buffer)."""
+    keep = []
+    views = _tensor_views(tensors, keep)
     h = C.c_void_p()
     check(load().sem_model_load(ctx.handle, C.byref(config), views, len(tensors), C.byref(h)))
     return Model(ctx, h)
@@ -273,4 +335,4 @@ class Q8Weight:
             pass
 
 
-__all__ = ["Model", "load_model", "load_model_from_views", "Q8Weight", "Context", "_lib"]
+__all__ = ["Model", "ModelAdapters", "load_model", "load_model_from_views", "Q8Weight", "Context", "_lib"]

@@ -42,6 +42,7 @@ typedef struct sem_group sem_group;
 typedef struct sem_adapter_plan sem_adapter_plan;
 typedef struct sem_lowrank sem_lowrank;
 typedef struct sem_block_norm sem_block_norm;
+typedef struct sem_model_adapters sem_model_adapters;
 
 /* Message of the last failed call on this thread (never NULL). A Go caller
  * holds its OS thread (runtime.LockOSThread) from the failing call until it
@@ -385,6 +386,42 @@ int sem_block_norm_free(sem_block_norm *b);
 int sem_block_norm_run(sem_block_norm *b, sem_adapter_plan *plan, int64_t rows, const void *d_o, int64_t ldo,
                        int32_t dtype, const void *d_h, int64_t ldh, int32_t h_dtype, void *d_h_out, int64_t ld_h_out,
                        void *d_y, int64_t ldy, void *stream);
+
+/* One adapter of a model: tensors named as in a GGUF adapter file,
+ *   blk.N.P.weight.lora_a {k_in, rank} and blk.N.P.weight.lora_b {rank, n_out}
+ * with P one of attn_q, attn_k, attn_v, attn_output, ffn_gate, ffn_up,
+ * ffn_down (type 0 F32, 1 F16 or 30 BF16; any subset of layers and
+ * projections, ranks 1..128), and, type F32, the gates and residual scales of
+ * a layer's two blocks,
+ *   blk.N.attn_residual.gate {embed_dim}, blk.N.attn_residual.scale {1},
+ *   blk.N.ffn_residual.gate {embed_dim}, blk.N.ffn_residual.scale {1}.
+ * The low-rank products are multiplied by alpha / rank (alpha 0: by 1). */
+typedef struct sem_adapter_view {
+  const sem_tensor_view *tensors;
+  int32_t n_tensors;
+  float alpha;
+} sem_adapter_view;
+
+/* Uploads n_adapters adapters of `model` (the caller's bytes may be released
+ * when the call returns); freed before the model. Errors: SEM_EFORMAT for a
+ * tensor with another name, shape or type, or a lora_a without its lora_b. */
+int sem_model_adapters_create(sem_model *model, const sem_adapter_view *adapters, int32_t n_adapters,
+                              sem_model_adapters **out);
+int sem_model_adapters_free(sem_model_adapters *adapters);
+
+/* sem_embed with an adapter for each sequence: use[s] an index, or -1 for the
+ * model as it is. One batch carries the sequences of many adapters; the base
+ * projections are shared. Every low-rank product reads the INT8 codes that the
+ * projection beside it reads, adds to its output before norm, attention or
+ * GELU, and a block's gate and residual scale apply where its post norm is
+ * added to the residual stream. Otherwise sem_embed's contract. A sequence
+ * with use[s] = -1 is embedded by the model as it is (where an adapter has a
+ * gate or residual scale, that layer's norm sums are float32 in another order
+ * for the whole batch); a batch of none but such runs sem_embed's forward. Not
+ * captured into the model's cached CUDA graphs.
+ * Further error: "adapter %d out of range (-1..%d)". */
+int sem_embed_adapted(sem_model *model, sem_model_adapters *adapters, const int32_t *ids, const int32_t *offsets,
+                      int32_t n_seqs, const int32_t *use, const int32_t *dims, float *out);
 
 /* ------------------------------------------------------------------------
  * Brute-force index: replaces search/brute (builder.go, index.go, storage.go).
