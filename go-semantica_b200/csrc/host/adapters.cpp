@@ -176,7 +176,6 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
   e = w->err.ensure(16);
   if (e != cudaSuccess) return set_error(SEM_ENOMEM, "device allocation failed: %s", cudaGetErrorString(e));
   std::vector<uint8_t> img(bytes, 0);
-  std::vector<LowRankAdapter> table(n_adapters);
   uint8_t* d = w->weights.as<uint8_t>();
   for (int32_t i = 0; i < n_adapters; ++i) {
     const int32_t r = ranks[i], rp = (int32_t)round_up(r, 8);
@@ -194,15 +193,14 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
                             r,
                             rp,
                             scales[i]};
-    table[i] = ad;
     std::memcpy(&img[(size_t)i * sizeof(LowRankAdapter)], &ad, sizeof ad);
   }
+  w->bank = LowRankBank{reinterpret_cast<const LowRankAdapter*>(d), n_adapters, k_in, n_out, ka, dtype, max_rank};
   std::lock_guard<std::mutex> lk(ctx->mu);
   if (bytes) SEM_CUDA(cudaMemcpyAsync(d, img.data(), bytes, cudaMemcpyHostToDevice, ctx->stream));
-  for (const LowRankAdapter& ad : table) SEM_CUDA(launch_lowrank_tiles(ad, k_in, n_out, ka, dtype, ctx->stream));
+  SEM_CUDA(launch_lowrank_tiles(w->bank, ctx->stream));
   SEM_CUDA(cudaMemsetAsync(w->err.p, 0, 16, ctx->stream));
   SEM_CUDA(cudaStreamSynchronize(ctx->stream));
-  w->bank = LowRankBank{reinterpret_cast<const LowRankAdapter*>(d), n_adapters, k_in, n_out, ka, dtype, max_rank};
   *out = w.release();
   return SEM_OK;
 }

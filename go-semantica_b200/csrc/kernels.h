@@ -330,12 +330,11 @@ cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& 
 cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
                               const LowRankArgs& args, uint32_t* err, cudaStream_t stream);
 // Bytes of an adapter's ta[xtype] and tb, whether it has unscale factors, and
-// the kernels that fill them from a and b.
+// the kernels that fill them from a and b for a whole bank.
 size_t lowrank_tile_bytes_a(int rank, int ka, int wtype, int xtype);
 size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype);
 inline bool lowrank_has_unscale(int wtype) { return wtype != kDtF16; }
-cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, int ka, int wtype,
-                                 cudaStream_t stream);
+cudaError_t launch_lowrank_tiles(const LowRankBank& bank, cudaStream_t stream);
 
 // h_out = scale * h + gate * (rmsnorm(o) * post), y = rmsnorm(h_out before its
 // rounding) * pre: gate and scale of the row's adapter (adapter 0 for every

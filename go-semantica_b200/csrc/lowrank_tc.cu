@@ -640,12 +640,20 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       if (!uc.next<true, true>(un, units, ufull, uempty, abort_flag, err)) break;
       --ahead;
       if (un.rank == 0) {
-        const int cols = min(n_out, un.c1 * 256) - un.c0 * 256;
+        // y = base, eight loads in flight per lane
+        const int first = un.c0 * 256, cols = min(n_out, un.c1 * 256) - first;
         for (int r = warp - kWarpEpi; r < un.rows; r += kEpiWarps) {
-          const int64_t row = p.plan.pos_row[un.pos0 + r];
-          for (int c = lane; c < cols; c += 32)
-            y[row * p.a.ldy + un.c0 * 256 + c] =
-                base ? base[row * p.a.ldb + un.c0 * 256 + c] : as_type<YT>(0.0f);
+          const int64_t row = un.row0 >= 0 ? un.row0 + r : p.plan.pos_row[un.pos0 + r];
+          const YT* src = base ? base + row * p.a.ldb + first : nullptr;
+          YT* dst = y + row * p.a.ldy + first;
+          for (int c = lane; c < cols; c += 256) {
+            YT v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = src ? src[min(c + 32 * j, cols - 1)] : as_type<YT>(0.0f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (c + 32 * j < cols) dst[c + 32 * j] = v[j];
+          }
         }
         continue;
       }
@@ -968,7 +976,9 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 // [chunk of 256 channels][even, odd][32 ranks][plane][128 rows], row i of a
 // chunk's tile g being channel 2 i + g.
 template <class WT>
-__global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int ka, int planes) {
+__global__ void lowrank_tiles_kernel(const LowRankAdapter* ads, int k_in, int n_out, int ka, int planes) {
+  const LowRankAdapter ad = ads[blockIdx.y];
+  if (ad.rank == 0) return;
   const int64_t na = (int64_t)ad.rank * ka;
   const int rcs = (ad.rp + KC - 1) / KC, tiles = (n_out + 255) / 256 * 2 * rcs;
   const int64_t nb = (int64_t)tiles * 128 * KC;
@@ -1010,9 +1020,11 @@ __global__ void lowrank_tiles_kernel(LowRankAdapter ad, int k_in, int n_out, int
 // the same way. A CTA per rank. fp16 parts of other types: the rank's weights
 // times the power of two that brings the largest to [2^13, 2^14).
 template <class WT>
-__global__ void lowrank_tiles16_kernel(LowRankAdapter ad, int k_in, int ka, int parts_f16, int parts_bf16) {
+__global__ void lowrank_tiles16_kernel(const LowRankAdapter* ads, int k_in, int ka, int parts_f16, int parts_bf16) {
   __shared__ float s_max[8];
+  const LowRankAdapter ad = ads[blockIdx.y];
   const int j = blockIdx.x;
+  if (j >= ad.rank) return;  // the whole CTA
   const WT* w = static_cast<const WT*>(ad.a) + (int64_t)j * ka;
   float top = 0.0f;
   for (int k = threadIdx.x; k < k_in; k += blockDim.x) top = fmaxf(top, fabsf(as_f32(w[k])));
@@ -1122,23 +1134,29 @@ size_t lowrank_tile_bytes_b(int rp, int n_out, int wtype) {
   return (size_t)((n_out + 255) / 256 * 2) * ((rp + KC - 1) / KC) * kBPlane * (wtype == kDtF32 ? 2 : 1);
 }
 
-cudaError_t launch_lowrank_tiles(const LowRankAdapter& ad, int k_in, int n_out, int ka, int wtype, cudaStream_t st) {
-  if (ad.rank <= 0) return cudaSuccess;
-  const int planes = wtype == kDtF32 ? 2 : 1;
-  const int64_t n = (int64_t)ad.rank * ka + (int64_t)((n_out + 255) / 256 * 2) * ((ad.rp + KC - 1) / KC) * 128 * KC;
-  const unsigned grid = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
-  const int f16 = a_parts(kDtF16, wtype), bf16 = a_parts(kDtBF16, wtype);
-  if (wtype == kDtF32) {
-    lowrank_tiles_kernel<float><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
-    lowrank_tiles16_kernel<float><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
-  } else if (wtype == kDtF16) {
-    lowrank_tiles_kernel<__half><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
-    lowrank_tiles16_kernel<__half><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
-  } else {
-    lowrank_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, k_in, n_out, ka, planes);
-    lowrank_tiles16_kernel<__nv_bfloat16><<<ad.rank, 256, 0, st>>>(ad, k_in, ka, f16, bf16);
+cudaError_t launch_lowrank_tiles(const LowRankBank& bank, cudaStream_t st) {
+  if (bank.max_rank <= 0) return cudaSuccess;
+  const int planes = bank.wtype == kDtF32 ? 2 : 1, rp = (bank.max_rank + 7) & ~7;
+  const int64_t n = (int64_t)bank.max_rank * bank.ka + (int64_t)((bank.n_out + 255) / 256 * 2) * ((rp + KC - 1) / KC) * 128 * KC;
+  const int f16 = a_parts(kDtF16, bank.wtype), bf16 = a_parts(kDtBF16, bank.wtype);
+  for (int at = 0; at < bank.n_adapters; at += 65535) {  // the grid's second dimension
+    const unsigned count = (unsigned)(bank.n_adapters - at < 65535 ? bank.n_adapters - at : 65535);
+    const dim3 grid((unsigned)((n + 1023) / 1024 < 256 ? (n + 1023) / 1024 : 256), count), grid16(bank.max_rank, count);
+    const LowRankAdapter* ads = bank.adapters + at;
+    if (bank.wtype == kDtF32) {
+      lowrank_tiles_kernel<float><<<grid, 256, 0, st>>>(ads, bank.k_in, bank.n_out, bank.ka, planes);
+      lowrank_tiles16_kernel<float><<<grid16, 256, 0, st>>>(ads, bank.k_in, bank.ka, f16, bf16);
+    } else if (bank.wtype == kDtF16) {
+      lowrank_tiles_kernel<__half><<<grid, 256, 0, st>>>(ads, bank.k_in, bank.n_out, bank.ka, planes);
+      lowrank_tiles16_kernel<__half><<<grid16, 256, 0, st>>>(ads, bank.k_in, bank.ka, f16, bf16);
+    } else {
+      lowrank_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ads, bank.k_in, bank.n_out, bank.ka, planes);
+      lowrank_tiles16_kernel<__nv_bfloat16><<<grid16, 256, 0, st>>>(ads, bank.k_in, bank.ka, f16, bf16);
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles, const LowRankArgs& a,
