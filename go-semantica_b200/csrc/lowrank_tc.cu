@@ -26,8 +26,8 @@
 //   - X warps (8): rows of x to where their operand goes, 128-byte swizzled:
 //     by TMA where a whole unit's rows follow each other, by asynchronous
 //     copies otherwise (any order and alignment); float32 is then split there;
-//   - two copy threads: the adapter's A and B tiles, which the bank keeps as
-//     tf32 planes in the swizzled layout, with one bulk copy per plane;
+//   - two copy threads: the adapter's A and B tiles, which the bank keeps in
+//     the swizzled layout, a bulk copy per piece (and the TMA of float32 x);
 //   - a shrink and an expand MMA thread, so that the shrink of later units
 //     goes on while the epilogue holds up the expand of an earlier one;
 //   - T warps (2): t from TMEM, scaled, split, to shared memory;
@@ -442,20 +442,21 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     int pending = 0;
     auto issue = [&]() {  // the cursor's stage, with one group of copies (an empty one by TMA, and at the end)
       if (more) {
-        ok = warp_wait(&xempty[ir.slot], ir.parity ^ 1, abort_flag, err, 1u);
-        if (!ok) return;
+        // float32 by TMA: the A thread loads it, the X warps take over when the bytes are there (xraw)
+        if (PX == 1 || tma_row < 0) {
+          ok = warp_wait(&xempty[ir.slot], ir.parity ^ 1, abort_flag, err, 1u);
+          if (!ok) return;
+        }
         uint8_t* dst = sX + ir.slot * x_slot;
         by_tma &= ~(1u << ir.slot);
         if (tma_row >= 0) {
           by_tma |= 1u << ir.slot;
-          // float32: the X warps take over when the bytes are there; 16-bit: they go straight to the MMAs
-          uint64_t* bar = PX == 2 ? &xraw[ir.slot] : &xfull[ir.slot];
-          if (elect_lane()) {
+          if (PX == 1 && elect_lane()) {  // 16-bit rows go straight to the MMAs
             if (warp == first_warp) {
-              mbar_arrive_expect_tx(bar, x_atom);
-              tma_load_2d(&p.tm_x, bar, dst, ks * KS, tma_row);
-            } else if (PX == 1) {
-              mbar_arrive(bar);
+              mbar_arrive_expect_tx(&xfull[ir.slot], x_atom);
+              tma_load_2d(&p.tm_x, &xfull[ir.slot], dst, ks * KS, tma_row);
+            } else {
+              mbar_arrive(&xfull[ir.slot]);
             }
           }
         } else {
@@ -940,8 +941,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     uint8_t* ring = is_a ? sA : sB;
     const uint32_t slots = is_a ? p.a_slots : p.b_slots, slot = is_a ? a_slot : kBPlane;
     uint64_t *full = is_a ? afull : bfull, *empty = is_a ? aempty : bempty;
-    Ring r;
-    uint32_t issued = 0;
+    Ring r, xr;
+    uint32_t issued = 0, x_issued = 0;
     bool ok = true;
     UnitCursor uc;
     Unit un;
@@ -950,7 +951,19 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int rcs = (un.rp + KC - 1) / KC;
       const uint32_t bytes = is_a ? un.rank * 128 : kBPlane;  // of a piece
       const uint8_t* src = is_a ? un.ta : un.tb + (size_t)un.c0 * 2 * rcs * PW * kBPlane;
-      for (int n = is_a ? k_stages * PA : (un.c1 - un.c0) * 2 * rcs * PW; n > 0; --n, src += bytes) {
+      const int pieces = is_a ? k_stages * PA : (un.c1 - un.c0) * 2 * rcs * PW;
+      const bool load_x = PX == 2 && is_a && p.x_vec && un.rows == p.rt && un.row0 >= 0;  // as the X warps see it
+      for (int n = 0; n < pieces; ++n, src += bytes) {
+        if (PX == 2 && is_a && n % PA == 0) {  // a stage of float32 rows
+          if (load_x) {
+            ok = stage_wait(&xempty[xr.slot], xr.parity ^ 1, abort_flag, err, 1u);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&xraw[xr.slot], x_atom);
+            tma_load_2d(&p.tm_x, &xraw[xr.slot], sX + xr.slot * x_slot, n / PA * KS, un.row0);
+          }
+          xr.next(p.x_slots);
+          ++x_issued;
+        }
         ok = stage_wait(&empty[r.slot], r.parity ^ 1, abort_flag, err, is_a ? 512u : 2048u);
         if (!ok) break;
         mbar_arrive_expect_tx(&full[r.slot], bytes);
@@ -962,6 +975,9 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     // copies in flight land before the CTA's shared memory is released
     for (uint32_t i = issued > slots ? issued - slots : 0; i < issued; ++i)
       mbar_wait_drain(&full[i % slots], (i / slots) & 1);
+    const uint32_t xs = p.x_slots;
+    for (uint32_t i = x_issued > xs ? x_issued - xs : 0; i < x_issued; ++i)
+      mbar_wait_drain(&xraw[i % xs], (i / xs) & 1);
   }
   }
   tc_fence_before();
