@@ -1,6 +1,6 @@
 // Adapters of many requests (sm_100a): the plan's row maps, the low-rank
-// adapters of small tiles on CUDA cores, and the block norm with its gate and
-// residual scale. The tensor-core kernel of the large tiles is lowrank_tc.cu.
+// adapters of small calls on CUDA cores, and the block norm with its gate and
+// residual scale. The tensor-core kernel is lowrank_tc.cu.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -142,15 +142,18 @@ __device__ __forceinline__ void load_row8(const T* p, int n, bool vec, float (&v
       load_vec<8>(p, v);
     }
   } else {
+    T e[8];  // all loads first: a condition or conversion in between would make each wait for the one before
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) e[i] = p[min(i, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(e[i]) : 0.0f;
   }
 }
 
 // RU: ranks per warp at most (ranks up to 8 RU).
 template <class XT, class YT, class WT, int RU>
 __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
-    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, int large_too, LowRankArgs a, int x_vec) {
+    lowrank_small_kernel(LowRankBank bank, AdapterPlanDev plan, LowRankArgs a, int x_vec) {
   extern __shared__ __align__(16) float smem[];
   float* s_x = smem;                                   // [16][kSmallLd]
   float* s_a = s_x + kSmallRows * kSmallLd;            // [rank][kSmallLd]
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
   bool started = false;  // every CTA of the cluster runs: its shared memory can be written
   cluster.barrier_arrive();
   const AdapterTile first = plan.small[min((int)(blockIdx.x / ctas), plan.max_seqs)];  // without waiting for the count
-  const int n_small = plan.counts[1], n_units = n_small + (large_too ? plan.counts[0] * kSubs : 0);
+  const int n_small = plan.counts[1], n_units = n_small + plan.counts[0] * kSubs;
 
   for (int u = (int)(blockIdx.x / ctas); u < n_units; u += (int)(gridDim.x / ctas)) {
     AdapterTile tl = first;
@@ -498,7 +501,7 @@ cudaError_t norm_types(const BlockNormArgs& a, cudaStream_t st) {
 }
 
 template <class XT, class YT, class WT, int RU>
-cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units, bool large_too,
+cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units,
                         const LowRankArgs& a, cudaStream_t st) {
   const int smem = small_smem_floats(bank.max_rank) * 4;
   if (smem > 48 * 1024) {
@@ -507,7 +510,7 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
     if (e != cudaSuccess) return e;
   }
   // the largest clusters whose CTAs are all on the device at once (three per SM; two at ranks above 32): 64 units of
-  // rank 16 take 20.5 us on clusters of eight, in two waves, and FOUR us on clusters of four
+  // rank 16 took 20.5 us on clusters of eight, in two waves, and take 13.1 us on clusters of four
   const int room = 132 * (RU <= 4 ? 3 : 2);
   const int ctas = n_units * 8 <= room ? 8 : n_units * 4 <= room ? 4 : 2;
   const int clusters = n_units < 2048 ? n_units : 2048;
@@ -522,17 +525,17 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, lowrank_small_kernel<XT, YT, WT, RU>, bank, plan, large_too ? 1 : 0, a,
+  return cudaLaunchKernelEx(&cfg, lowrank_small_kernel<XT, YT, WT, RU>, bank, plan, a,
                             aligned16(a.x, a.ldx, sizeof(XT)) ? 1 : 0);
 }
 template <class XT, class YT>
-cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units, bool large_too,
+cudaError_t small_types(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units,
                         const LowRankArgs& a, cudaStream_t st) {
   auto pick = [&](auto w) {
     using WT = decltype(w);
-    if (bank.max_rank <= 16) return small_ranks<XT, YT, WT, 2>(bank, plan, n_units, large_too, a, st);
-    if (bank.max_rank <= 32) return small_ranks<XT, YT, WT, 4>(bank, plan, n_units, large_too, a, st);
-    return small_ranks<XT, YT, WT, 16>(bank, plan, n_units, large_too, a, st);
+    if (bank.max_rank <= 16) return small_ranks<XT, YT, WT, 2>(bank, plan, n_units, a, st);
+    if (bank.max_rank <= 32) return small_ranks<XT, YT, WT, 4>(bank, plan, n_units, a, st);
+    return small_ranks<XT, YT, WT, 16>(bank, plan, n_units, a, st);
   };
   return bank.wtype == kDtF32 ? pick(float()) : pick(uint16_t());
 }
@@ -548,18 +551,18 @@ cudaError_t launch_adapter_plan(const int32_t* pos, const int32_t* row0, const i
   return cudaGetLastError();
 }
 
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_small, int n_large,
-                                 bool large_too, const LowRankArgs& a, cudaStream_t st) {
-  const int64_t units = (int64_t)n_small + (large_too ? (int64_t)n_large * (kAdapterTileRows / kSmallRows) : 0);
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_large, int n_small,
+                                 const LowRankArgs& a, cudaStream_t st) {
+  const int64_t units = (int64_t)n_small + (int64_t)n_large * (kAdapterTileRows / kSmallRows);
   if (units <= 0) return cudaSuccess;
   const int n = units < 0x7fffffff ? (int)units : 0x7fffffff;
-  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, n, large_too, a, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF16) return small_types<__half, __half>(bank, plan, n, large_too, a, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF32) return small_types<__half, float>(bank, plan, n, large_too, a, st);
+  if (a.xtype == kDtF32 && a.ytype == kDtF32) return small_types<float, float>(bank, plan, n, a, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF16) return small_types<__half, __half>(bank, plan, n, a, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF32) return small_types<__half, float>(bank, plan, n, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtBF16)
-    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, n, large_too, a, st);
+    return small_types<__nv_bfloat16, __nv_bfloat16>(bank, plan, n, a, st);
   if (a.xtype == kDtBF16 && a.ytype == kDtF32)
-    return small_types<__nv_bfloat16, float>(bank, plan, n, large_too, a, st);
+    return small_types<__nv_bfloat16, float>(bank, plan, n, a, st);
   return cudaErrorInvalidValue;
 }
 

@@ -118,6 +118,8 @@ int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapter
                                maps, maps + p->max_rows, maps + 2 * p->max_rows, st));
   p->n_large = (int32_t)h.large.size();
   p->n_small = (int32_t)h.small.size();
+  p->small_rows = 0;
+  for (const AdapterTile& t : h.small) p->small_rows += t.rows;
   p->rows = h.rows;
   p->n_seqs = n_seqs;
   p->max_adapter = h.max_adapter;
@@ -227,22 +229,24 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, const LowRankArgs& ar
 // tensor-core kernel's pipeline takes longer to fill than they take. Measured
 // (CUDA cores / tensor cores, 768 x 768, rank 16): INT8 codes 12.6 M 8.3 / 12.0
 // us, 25 M 12.0 / 13.4, 50 M 18.7 / 14.5; float32 rows, whose conversion the
-// tensor cores wait for, 25 M 11.3 / 20.7; 517 x 1001, 168 M 48.8 / 49.9.
+// tensor cores wait for, 25 M 11.3 / 19.9; 517 x 1001, 168 M 48.7 / 44.8. A tile
+// of up to 16 rows counts as eight (256 single fp16 rows of as many adapters:
+// 33.3 / 25.0 us; 64 tiles of 12 rows: 13.1 on the CUDA cores).
 constexpr int64_t kLowRankSmallWork = 28000000, kLowRankSmallWorkF32 = 80000000;
 
-// Both tile lists of the plan. A captured launch may be replayed with a plan
-// set to another batch, so a capture records a launch for each list.
+// One launch for all tiles of the plan, also for an empty plan when it is
+// captured (a replay may find the plan set to another batch).
 int lowrank_enqueue(const LowRankBank& bank, const sem_adapter_plan* plan, const LowRankArgs& args, bool captured,
                     uint32_t* err, cudaStream_t st) {
   const AdapterPlanDev dev = plan_device(plan);
-  const int64_t work = (int64_t)plan->rows * bank.max_rank * (bank.k_in + bank.n_out);
+  const int64_t rows = (int64_t)plan->rows - plan->small_rows + 8 * (int64_t)plan->n_small;
+  const int64_t work = rows * bank.max_rank * (bank.k_in + bank.n_out);
   const int path = get_lowrank_path();
   const bool cuda_cores = path == SEM_LOWRANK_PATH_CUDA_CORES || (path == SEM_LOWRANK_PATH_AUTO && work <= (args.xtype == kDtF32 ? kLowRankSmallWorkF32 : kLowRankSmallWork));
-  if (!cuda_cores && (plan->n_large > 0 || captured))
-    SEM_CUDA(launch_lowrank_tc(bank, dev, plan->n_large > 0 ? plan->n_large : 1, args, err, st));
-  if (plan->n_small > 0 || (cuda_cores && plan->n_large > 0) || captured)
-    SEM_CUDA(launch_lowrank_small(bank, dev, plan->n_small > 0 || plan->n_large > 0 ? plan->n_small : 1,
-                                  plan->n_large, cuda_cores, args, st));
+  if (plan->rows == 0 && !captured) return SEM_OK;
+  const int n_large = plan->n_large, n_small = n_large || plan->n_small ? plan->n_small : 1;
+  if (cuda_cores) SEM_CUDA(launch_lowrank_small(bank, dev, n_large, n_small, args, st));
+  else SEM_CUDA(launch_lowrank_tc(bank, dev, n_large, n_small, args, err, st));
   return SEM_OK;
 }
 

@@ -8,7 +8,7 @@ struct sem_adapter_plan {
   int64_t max_rows = 0;
   int32_t max_seqs = 0;
   std::mutex mu;            // the host fields below, and set against use
-  int32_t n_large = 0, n_small = 0, rows = 0, n_seqs = 0, max_adapter = -1;
+  int32_t n_large = 0, n_small = 0, small_rows = 0, rows = 0, n_seqs = 0, max_adapter = -1;
   sem::DevBuf up;           // counts, sorted sequences, tiles (uploaded)
   sem::DevBuf maps;         // pos_row, pos_seq, row_adapter [max_rows] each
   sem::HostBuf staging;     // the upload's pinned image

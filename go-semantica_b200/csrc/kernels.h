@@ -321,13 +321,13 @@ struct LowRankArgs {
   const uint32_t* absmax;
   int32_t per_seq;
 };
-// The plan's small tiles, and with large_too its large ones, on CUDA cores
-// (adapters.cu).
-cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_small, int n_large,
-                                 bool large_too, const LowRankArgs& args, cudaStream_t stream);
-// The large tiles on the tensor cores (lowrank_tc.cu). `err` (nullable)
-// receives error bits if a pipeline wait times out.
-cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles,
+// All tiles of the plan (n_large and n_small size the launch; the kernels read
+// the counts on the device) on CUDA cores (adapters.cu)
+cudaError_t launch_lowrank_small(const LowRankBank& bank, const AdapterPlanDev& plan, int n_large, int n_small,
+                                 const LowRankArgs& args, cudaStream_t stream);
+// or on the tensor cores (lowrank_tc.cu). `err` (nullable) receives error bits
+// if a pipeline wait times out.
+cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_large, int n_small,
                               const LowRankArgs& args, uint32_t* err, cudaStream_t stream);
 // Bytes of an adapter's ta[xtype] and tb, whether it has unscale factors, and
 // the kernels that fill them from a and b for a whole bank.

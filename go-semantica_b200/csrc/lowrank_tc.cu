@@ -1,4 +1,4 @@
-// Low-rank adapters of large tiles on the sm_100a tensor cores.
+// Low-rank adapters on the sm_100a tensor cores.
 //
 //   y[row] = base[row] + s (x[row] A^T) B^T
 //
@@ -36,7 +36,7 @@
 //     ahead of the accumulators and across units.
 // One persistent CTA per SM. Loads into registers in place of the asynchronous
 // copies were measured: what is in flight then has to fit the 20-odd KB of L1
-// that the shared memory leaves, 148 us against MEAS_NEW (128 x 512 rows).
+// that the shared memory leaves.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -196,6 +196,21 @@ __device__ __forceinline__ T as_type(float v) {
   else return __float2bfloat16_rn(v);
 }
 
+template <class T>
+__device__ __forceinline__ uint32_t raw_bits(T v) {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(v);
+  else return *reinterpret_cast<const uint16_t*>(&v);
+}
+template <class T>
+__device__ __forceinline__ T from_bits(uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(b);
+  } else {
+    const uint16_t h = (uint16_t)b;
+    return *reinterpret_cast<const T*>(&h);
+  }
+}
+
 // 32 lanes x 8 columns of TMEM.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -263,20 +278,25 @@ struct TcParams {
   int32_t x_slots, a_slots, b_slots, t_bufs;  // ring depths
   int32_t epi_ring;  // bytes of an epilogue warp's ring: 2048 or 4096
   int32_t x_vec;   // rows of x start on 16 bytes (16-byte copies, TMA)
+  int32_t x_four;  // rows of x start on 4 bytes
   int32_t b_copy;  // bytes of a copy that base's rows are aligned for: 16, 4 or 2 (none, element loads)
   int32_t y_pair;  // y's channels can be stored in pairs
   uint32_t* err;
 };
 
-// Unit u. Sub-tiles of the same number lie together, so that those behind a
-// tile's last row come last.
+// Units of the plan's tiles: large ones in parts of rt rows, parts of the same
+// number together (so that those behind a tile's last row come last), then the
+// small ones.
+__device__ __forceinline__ int64_t count_units(const TcParams& p, int n_large, int n_small) {
+  return ((int64_t)n_large * (kAdapterTileRows / p.rt) + n_small) * p.splits;
+}
 template <int XTYPE>
-__device__ __forceinline__ Unit get_unit(const TcParams& p, int n_tiles, int64_t u) {
+__device__ __forceinline__ Unit get_unit(const TcParams& p, int n_large, int64_t u) {
   Unit r;
   const int split = (int)(u % p.splits);
-  const int64_t v = u / p.splits;
-  const AdapterTile tl = p.plan.large[v % n_tiles];
-  const int off = (int)(v / n_tiles) * p.rt;
+  const int64_t v = u / p.splits, small = v - (int64_t)n_large * (kAdapterTileRows / p.rt);
+  const AdapterTile tl = small >= 0 ? p.plan.small[small] : p.plan.large[v % n_large];
+  const int off = small >= 0 ? 0 : (int)(v / n_large) * p.rt;
   r.pos0 = tl.pos0 + off;
   r.rows = min(p.rt, tl.rows - off);
   r.row0 = tl.row0 < 0 ? -1 : tl.row0 + off;
@@ -465,22 +485,25 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 #pragma unroll
           for (int i = 0; i < XV; ++i) {
             if (i >= passes || r0 + i * XR >= p.rt) break;
+            const uint32_t d = smem_u32(dst) + at0 + i * XR * 128;
             if (ks < full_stages) {
-              copy16(smem_u32(dst) + at0 + i * XR * 128, row[i] + ks * KS, 16);
-            } else {
-              XT e[XE];  // channels behind the last: zeros (that A's are zeros is not enough for a NaN)
+              copy16(d, row[i] + ks * KS, 16);
+            } else if (p.x_four) {  // what lies behind k is zeros (that A's are zeros is not enough for a NaN)
+              constexpr int E4 = 4 / sizeof(XT);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int bytes = max(0, min(4, (k - c - j * E4) * (int)sizeof(XT)));
+                copy4(d + j * 4, row[i] + (bytes ? ks * KS + j * E4 : -col), bytes);
+              }
+            } else if constexpr (PX == 1) {  // odd 16-bit addresses: loads, clamped instead of conditional
+              XT e[XE];
 #pragma unroll
               for (int j = 0; j < XE; ++j) e[j] = row[i][min(c + j, k - 1) - col];
               uint32_t v[4];
-              if constexpr (PX == 2) {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = c + j < k ? __float_as_uint(e[j]) : 0u;
-              } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(e);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  v[j] = (c + 2 * j < k ? h[2 * j] : 0u) | (c + 2 * j + 1 < k ? (uint32_t)h[2 * j + 1] << 16 : 0u);
-              }
+              for (int j = 0; j < 4; ++j)
+                v[j] = (c + 2 * j < k ? h[2 * j] : 0u) | (c + 2 * j + 1 < k ? (uint32_t)h[2 * j + 1] << 16 : 0u);
               *reinterpret_cast<uint4*>(dst + at0 + i * XR * 128) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -701,24 +724,42 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             b[j].e[0] = as_type<YT>(__fadd_rn(as_f32(b[j].e[0]), __uint_as_float(v0[j])));
             b[j].e[1] = as_type<YT>(__fadd_rn(as_f32(b[j].e[1]), __uint_as_float(v1[j])));
           }
-          if (p.y_pair && un.row0 >= 0 && i + S <= i1) {  // the usual case in few instructions
-            if (ch < n_out) {
-              YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + ch;
+          const bool whole = un.row0 >= 0 && i + S <= i1;  // the usual case in few instructions
+          if (p.y_pair) {
+            if (whole) {
+              if (ch < n_out) {
+                YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + ch;
 #pragma unroll
-              for (int j = 0; j < S; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
+                for (int j = 0; j < S; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < S; ++j) {
+                const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
+                if (i + j < i1 && ch < n_out) *reinterpret_cast<Pair*>(y + (int64_t)row * p.a.ldy + ch) = b[j];
+              }
             }
           } else {
+            // single values: exchanged so that the lanes' channels follow each other, lane and lane + 32
+            const int c0 = ch - lane;
+            auto swap = [&](int from, const Pair& v) -> YT {
+              const uint32_t bits = __shfl_sync(0xffffffffu, raw_bits(v.e[0]), from);
+              const uint32_t odd = __shfl_sync(0xffffffffu, raw_bits(v.e[1]), from);
+              return from_bits<YT>(lane & 1 ? odd : bits);
+            };
+            YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + c0;
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-              const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
-              if (i + j >= i1) continue;
-              YT* dst = y + (int64_t)row * p.a.ldy + ch;
-              if (p.y_pair) {
-                if (ch < n_out) *reinterpret_cast<Pair*>(dst) = b[j];
-              } else {
-                if (ch < n_out) dst[0] = b[j].e[0];
-                if (ch + 1 < n_out) dst[1] = b[j].e[1];
+              const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
+              if (!whole) {
+                const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
+                dst = y + (int64_t)row * p.a.ldy + c0;
               }
+              if (i + j < i1) {
+                if (c0 < n_out) dst[0] = lo;
+                if (c0 + 32 < n_out) dst[32] = hi;
+              }
+              dst += p.a.ldy;
             }
           }
         }
@@ -907,8 +948,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     }
   } else if (warp == kWarpUnits) {
     // ---------------- units: looked up 32 at a time ----------------
-    const int n_tiles = p.plan.counts[0];
-    const int64_t n_units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
+    const int n_large = p.plan.counts[0];
+    const int64_t n_units = count_units(p, n_large, p.plan.counts[1]);
     const bool in_place = p.a.base == p.a.y && p.a.ldb == p.a.ldy;  // nothing to do for rows without an adapter
     Ring r;
     bool ok = true;
@@ -916,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       const int64_t u = first + lane * (int64_t)gridDim.x;
       Unit un;
       un.rows = 0;
-      if (u < n_units) un = get_unit<XTYPE>(p, n_tiles, u);
+      if (u < n_units) un = get_unit<XTYPE>(p, n_large, u);
       uint32_t todo = __ballot_sync(0xffffffffu, un.rows > 0 && un.c1 > un.c0 && (un.rank > 0 || !in_place));
       const bool last = first + 32 * (int64_t)gridDim.x >= n_units;
       while (ok && (todo || last)) {
@@ -1076,7 +1117,7 @@ __global__ void lowrank_tiles16_kernel(const LowRankAdapter* ads, int k_in, int 
 }
 
 template <class XT, class YT>
-cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
+cudaError_t tc_types(TcParams p, int n_large, int n_small, cudaStream_t st) {
   constexpr int XTYPE = dtype_of<XT>(), PX = XTYPE == kDtF32 ? 2 : 1;
   const int chunks = (p.bank.n_out + 255) / 256;
   int dev = 0, sms = 0;
@@ -1085,8 +1126,12 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   p.rt = kRt;
   p.splits = 1;
-  while (p.rt > 16 && (int64_t)n_tiles * (kAdapterTileRows / p.rt) < sms) p.rt /= 2;
-  while (p.splits < chunks && (int64_t)n_tiles * (kAdapterTileRows / p.rt) * (p.splits + 1) <= sms) ++p.splits;
+  // Fewer rows per unit, then shares of the channels, while all units still run at once: a unit's time is mostly its
+  // pipeline's latency (6075 ragged float32 rows, 512 x 1024, rank 23: 36.5 us in one round of 64-row units, 39.6 in
+  // two rounds of 32).
+  auto units = [&](int rt, int splits) { return ((int64_t)n_large * (kAdapterTileRows / rt) + n_small) * splits; };
+  while (p.rt > 16 && units(p.rt / 2, 1) <= sms) p.rt /= 2;
+  while (p.splits < chunks && units(p.rt, p.splits + 1) <= sms) ++p.splits;
   // Shared memory: the most rows that fit two slots of every ring, then what is left for more of them.
   const int t_chunks = (p.bank.max_rank + KC - 1) / KC, a_slot = (p.bank.max_rank + 15) / 16 * 16 * 128;
   int smem = 0;
@@ -1114,6 +1159,7 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   }
   if (!smem) return cudaErrorInvalidValue;
   p.x_vec = (reinterpret_cast<uintptr_t>(p.a.x) & 15) == 0 && (p.a.ldx * sizeof(XT)) % 16 == 0;
+  p.x_four = (reinterpret_cast<uintptr_t>(p.a.x) | (uint64_t)(p.a.ldx * sizeof(XT))) % 4 == 0;
   const uintptr_t base = reinterpret_cast<uintptr_t>(p.a.base);
   p.b_copy = (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 16 == 0 ? 16
              : (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 4 == 0 ? 4 : 2;
@@ -1136,8 +1182,8 @@ cudaError_t tc_types(TcParams p, int n_tiles, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(lowrank_tc_kernel<XT, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
-  const int64_t units = (int64_t)n_tiles * (kAdapterTileRows / p.rt) * p.splits;
-  lowrank_tc_kernel<XT, YT><<<(unsigned)(units < sms ? units : sms), kThreads, smem, st>>>(p);
+  const int64_t n = units(p.rt, p.splits);
+  lowrank_tc_kernel<XT, YT><<<(unsigned)(n < sms ? n : sms), kThreads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1175,19 +1221,19 @@ cudaError_t launch_lowrank_tiles(const LowRankBank& bank, cudaStream_t st) {
   return cudaSuccess;
 }
 
-cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_tiles, const LowRankArgs& a,
-                              uint32_t* err, cudaStream_t st) {
-  if (n_tiles <= 0) return cudaSuccess;
+cudaError_t launch_lowrank_tc(const LowRankBank& bank, const AdapterPlanDev& plan, int n_large, int n_small,
+                              const LowRankArgs& a, uint32_t* err, cudaStream_t st) {
+  if (n_large <= 0 && n_small <= 0) return cudaSuccess;
   TcParams p{};
   p.bank = bank;
   p.plan = plan;
   p.a = a;
   p.err = err;
-  if (a.xtype == kDtF32 && a.ytype == kDtF32) return tc_types<float, float>(p, n_tiles, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF16) return tc_types<__half, __half>(p, n_tiles, st);
-  if (a.xtype == kDtF16 && a.ytype == kDtF32) return tc_types<__half, float>(p, n_tiles, st);
-  if (a.xtype == kDtBF16 && a.ytype == kDtBF16) return tc_types<__nv_bfloat16, __nv_bfloat16>(p, n_tiles, st);
-  if (a.xtype == kDtBF16 && a.ytype == kDtF32) return tc_types<__nv_bfloat16, float>(p, n_tiles, st);
+  if (a.xtype == kDtF32 && a.ytype == kDtF32) return tc_types<float, float>(p, n_large, n_small, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF16) return tc_types<__half, __half>(p, n_large, n_small, st);
+  if (a.xtype == kDtF16 && a.ytype == kDtF32) return tc_types<__half, float>(p, n_large, n_small, st);
+  if (a.xtype == kDtBF16 && a.ytype == kDtBF16) return tc_types<__nv_bfloat16, __nv_bfloat16>(p, n_large, n_small, st);
+  if (a.xtype == kDtBF16 && a.ytype == kDtF32) return tc_types<__nv_bfloat16, float>(p, n_large, n_small, st);
   return cudaErrorInvalidValue;
 }
 

@@ -351,8 +351,7 @@ int sem_lowrank_apply(sem_lowrank *w, sem_adapter_plan *plan, const void *d_x, i
 int sem_lowrank_apply_int8(sem_lowrank *w, sem_adapter_plan *plan, const void *d_codes, const uint32_t *d_absmax,
                            int32_t n_absmax, const float *d_base, int64_t ld_base, float *d_y, int64_t ldy,
                            void *stream);
-/* Which kernel takes the groups of more than 16 rows of one adapter
- * (process-wide; smaller groups always run on the CUDA cores, in float32):
+/* Which kernel runs the low-rank products (process-wide):
  *   SEM_LOWRANK_PATH_AUTO (default): the tensor cores, or the CUDA cores where
  *     the whole call is too little work to fill the tensor cores' pipeline;
  *   SEM_LOWRANK_PATH_CUDA_CORES, SEM_LOWRANK_PATH_TENSOR: always these.
