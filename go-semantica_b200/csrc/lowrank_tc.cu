@@ -54,11 +54,17 @@ constexpr int kXWarps = 8, kXGroups = 2, kEpiWarps = 16, kTWarps = 2;
 constexpr int kWarpEpi = kXWarps, kWarpT = kWarpEpi + kEpiWarps, kWarpShrink = kWarpT + kTWarps;
 constexpr int kWarpA = kWarpShrink + 1, kWarpExpand = kWarpA + 1, kWarpB = kWarpExpand + 1, kWarpUnits = kWarpB + 1;
 constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups: T, MMA, copy and unit warps, one idle
-// Registers: 1024 threads get 64 each at launch; the last two warpgroups give
-// some back (setmaxnreg) to the x and the epilogue warpgroups, which would
-// spill otherwise, into an L1 that the shared memory leaves too small for it.
-constexpr int kRegsX = 72, kRegsEpi = 72, kRegsRest = 40;
-static_assert(kThreads == 1024 && kXWarps * kRegsX + kEpiWarps * kRegsEpi + 8 * kRegsRest <= 32 * 64, "register split");
+// Registers: 1024 threads get 64 each at launch; the last two warpgroups (and
+// the X warps of 16-bit rows, which split nothing) give some back to the
+// epilogue's. The shared memory leaves the L1 too small for spills: with
+// 12 to 60 bytes of them (72, 72 and 40 registers) 102 thousand bf16 rows,
+// 768 x 2304, rank to 64, took 367 us instead of 306.
+template <class XT>
+struct Regs {
+  static constexpr int x = sizeof(XT) == 4 ? 64 : 48, epi = sizeof(XT) == 4 ? 72 : 80, rest = 48;
+  static_assert(kXWarps * x + kEpiWarps * epi + 8 * rest <= kThreads / 32 * 64, "register split");
+};
+static_assert(kThreads == 1024, "64 registers at launch");
 static_assert(kWarpEpi % 4 == 0 && kWarpT % 4 == 0, "TMEM lane quarters go by warp index");
 constexpr int KC = 32;   // tf32 per swizzled 128-byte row
 constexpr int kRt = 64;  // rows per unit at most
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 
   if (warp < kXWarps) {
     // ---------------- x: global -> swizzled shared memory; float32 split in place ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsX));
+    if constexpr (Regs<XT>::x < 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<XT>::x));
     const int k = p.bank.k_in;
     // The two groups of warps take the stages in turn (counted over all units), so that one converts while the other
     // waits, fences and issues.
@@ -554,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       mbar_wait_drain(PX == 2 ? &xraw[xr.slot] : &xfull[xr.slot], xr.parity);
   } else if (warp < kWarpT) {
     // ---------------- epilogue: base + accumulators -> y ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<XT>::epi));
     struct alignas(2 * sizeof(YT)) Pair { YT e[2]; };
     constexpr int B = epi_rows<YT>(), RB = 64 * sizeof(YT);  // rows of a batch, bytes of one: this warp's 64 channels
     constexpr int S = 8;                                     // rows in registers
@@ -772,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     cp_async_wait<0>();
     for (; !ok && filled > 0; --filled, er.next(nb)) mbar_wait_drain(&bars[er.slot], er.parity);  // as above
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<XT>::rest));
     if (warp < kWarpShrink) {
     // ---------------- t: TMEM -> scaled, split -> shared memory ----------------
     const int quarter = warp & 3, row = quarter * 32 + lane;  // this lane's row of the unit
