@@ -509,10 +509,11 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
         cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  // the largest clusters whose CTAs are all on the device at once (three per SM; two at ranks above 32): 64 units of
-  // rank 16 took 20.5 us on clusters of eight, in two waves, and take 13.1 us on clusters of four
+  // the largest clusters whose CTAs are all on the device at once (three per SM, two at ranks above 32; 132 SMs, since
+  // a cluster of eight leaves some of a processing cluster's unused): 64 units of rank 16 took 20.5 us on clusters of
+  // eight, in two waves, and take 13.1 us on clusters of four
   const int room = 132 * (RU <= 4 ? 3 : 2);
-  const int ctas = n_units * 8 <= room ? 8 : n_units * 4 <= room ? 4 : 2;
+  const int ctas = n_units <= room / 8 ? 8 : n_units <= room / 4 ? 4 : 2;
   const int clusters = n_units < 2048 ? n_units : 2048;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(clusters * ctas));

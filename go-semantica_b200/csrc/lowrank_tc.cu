@@ -1177,10 +1177,11 @@ cudaError_t tc_types(TcParams p, int n_large, int n_small, cudaStream_t st) {
     break;
   }
   if (!smem) return cudaErrorInvalidValue;
-  p.x_vec = (reinterpret_cast<uintptr_t>(p.a.x) & 15) == 0 && (p.a.ldx * sizeof(XT)) % 16 == 0;
+  constexpr int64_t kMaxLd = 1ll << 37;  // a tensor map's strides are below 2^40 bytes (a single row can have any)
+  p.x_vec = (reinterpret_cast<uintptr_t>(p.a.x) & 15) == 0 && (p.a.ldx * sizeof(XT)) % 16 == 0 && p.a.ldx <= kMaxLd;
   p.x_four = (reinterpret_cast<uintptr_t>(p.a.x) | (uint64_t)(p.a.ldx * sizeof(XT))) % 4 == 0;
   const uintptr_t base = reinterpret_cast<uintptr_t>(p.a.base);
-  p.b_copy = (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 16 == 0 ? 16
+  p.b_copy = (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 16 == 0 && p.a.ldb <= kMaxLd ? 16
              : (base | (uint64_t)(p.a.ldb * sizeof(YT))) % 4 == 0 ? 4 : 2;
   p.y_pair = p.bank.n_out % 2 == 0 &&
              (reinterpret_cast<uintptr_t>(p.a.y) | (uint64_t)(p.a.ldy * sizeof(YT))) % (2 * sizeof(YT)) == 0;

@@ -84,6 +84,8 @@ class Model:
         elif np.isscalar(dims):
             dims = [int(dims)] * n
         d = np.ascontiguousarray(dims, dtype=np.int32)
+        if d.size != n:
+            raise ValueError(f"{d.size} output widths for {n} sequences")
         out = np.empty(max(int(d[d > 0].sum()) if n else 0, 1), dtype=np.float32)
         check(load().sem_embed_adapted(self.handle, adapters.handle, ids.ctypes.data, offsets.ctypes.data, n,
                                        use.ctypes.data, d.ctypes.data, out.ctypes.data))

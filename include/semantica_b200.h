@@ -380,8 +380,9 @@ int sem_block_norm_free(sem_block_norm *b);
  * rmsnorm(v) = v / sqrt(mean(v^2) + eps), in float32; o itself without
  * post_w, no y (d_y is not used) without pre_w. o and y are of type dtype, h
  * and h_out of type h_dtype (dtype, or F32). h_out may be h, y may be o; no
- * other overlap. `rows` is the plan's row count when there is a plan. Strides
- * as for sem_lowrank_apply. */
+ * other overlap. `rows` is the plan's row count when there is a plan; a
+ * captured call keeps it, so its plan may be set to batches of that many rows.
+ * Strides as for sem_lowrank_apply. */
 int sem_block_norm_run(sem_block_norm *b, sem_adapter_plan *plan, int64_t rows, const void *d_o, int64_t ldo,
                        int32_t dtype, const void *d_h, int64_t ldh, int32_t h_dtype, void *d_h_out, int64_t ld_h_out,
                        void *d_y, int64_t ldy, void *stream);

@@ -359,6 +359,39 @@ def test_lowrank_strides_and_base(ctx, path, pads, base, x, y):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("x,y", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("start", [1, 2, 4])
+def test_lowrank_rows_from_any_element(ctx, path, start, x, y):
+    # strides of whole 16-byte pieces, but rows that start `start` elements behind one
+    import torch
+    c = LowRankCase(ctx, [3, 60, 140], [0, 1, 2], [8, 24, 40], 72, 136, x=x, y=y, pads=(8, 8, 8))
+
+    def moved(t):
+        wide = torch.empty(t.numel() + start, dtype=t.dtype, device="cuda")
+        wide[start:] = t.flatten()
+        return wide[start:].view(t.shape)
+
+    c.dx, c.dbase, c.dy = moved(c.dx), moved(c.dbase), moved(c.dy)
+    c.run(ctx)
+    c.run(ctx, "y")
+    c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,y", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("ld", [2 ** 37, 2 ** 40, 2 ** 40 + 1])
+def test_lowrank_single_row_of_any_stride(ctx, path, ld, x, y):
+    # no second row is there to be read at the stride
+    import torch
+    c = LowRankCase(ctx, [1], [0], [24], 72, 136, x=x, y=y)
+    c.bank.apply(c.plan, c.dx.data_ptr(), DT[x], c.dy.data_ptr(), DT[y], c.dbase.data_ptr(), ld, ld, ld, ctx.stream)
+    c.bank.check()
+    c.verify(c.dy)
+    torch.cuda.synchronize()
+    c.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("codes", [1, 2])
 @pytest.mark.parametrize("w", ["f16", "f32"])
 def test_lowrank_int8_codes(ctx, path, codes, w):

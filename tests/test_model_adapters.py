@@ -248,6 +248,8 @@ def test_adapter_refusals(model, ctx, tensors):
             model.forward_batch_adapted(ad, ids, offs, use)
     with pytest.raises(ValueError, match="1 adapters for 2 sequences"):
         model.forward_batch_adapted(ad, ids, offs, [0])
+    with pytest.raises(ValueError, match="1 output widths for 2 sequences"):
+        model.forward_batch_adapted(ad, ids, offs, [0, 0], [128])
     with pytest.raises(_lib.SemError, match="empty input"):
         model.forward_batch_adapted(ad, ids, np.array([0, 3, 3], np.int32), [0, 0])
     with pytest.raises(_lib.SemError, match="token ID out of range"):
