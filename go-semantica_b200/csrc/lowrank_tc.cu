@@ -38,7 +38,7 @@
 // rate of a plain copy, in parentheses):
 //   65536 float32 rows, 768 x 768, rank 16:             114 us (92)
 //   196608 rows of codes, 1152 x 768, rank 32:          285 us (253)
-//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    307 us (181)
+//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    314 us (181)
 //   16384 fp16 rows, 768 x 1280, rank 128, f32 weights:  93 us (17)
 //   6075 ragged float32 rows, 517 x 1001, rank to 23:    45 us (9)
 // The first two are near the copy's rate. In the third a unit reads 0.6 MB of
@@ -66,7 +66,7 @@ constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups
 // the X warps of 16-bit rows, which split nothing) give some back to the
 // epilogue's. The shared memory leaves the L1 too small for spills: with
 // 12 to 60 bytes of them (72, 72 and 40 registers) 102 thousand bf16 rows,
-// 768 x 2304, rank to 64, took 367 us instead of 306.
+// 768 x 2304, rank to 64, took 365 us and takes 306 without.
 template <class XT>
 struct Regs {
   static constexpr int x = sizeof(XT) == 4 ? 64 : 48, epi = sizeof(XT) == 4 ? 72 : 80, rest = 48;
@@ -716,12 +716,6 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             const uint8_t* src = sE + (ring - smem_u32(sE)) + (er.slot * B + sub) * RB + lane * 2 * sizeof(YT);
 #pragma unroll
             for (int j = 0; j < S; ++j) b[j] = *reinterpret_cast<const Pair*>(src + j * RB);
-            if (sub + S == B || i + S >= i1) {
-              er.next(nb);
-              --filled;
-              __syncwarp();
-              fill();
-            }
           } else {
 #pragma unroll
             for (int j = 0; j < S; ++j) b[j].e[0] = b[j].e[1] = as_type<YT>(0.0f);
@@ -736,6 +730,15 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           for (int j = 0; j < S; ++j) {
             b[j].e[0] = as_type<YT>(__fadd_rn(as_f32(b[j].e[0]), __uint_as_float(v0[j])));
             b[j].e[1] = as_type<YT>(__fadd_rn(as_f32(b[j].e[1]), __uint_as_float(v1[j])));
+          }
+          // The slot's next copy: the sums hold its values, and the fence orders the loads before what TMA writes. (Right
+          // behind the loads nothing makes a copy wait for them.)
+          if (base && (sub + S == B || i + S >= i1)) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            er.next(nb);
+            --filled;
+            fill();
           }
           const bool whole = un.row0 >= 0 && i + S <= i1;  // the usual case in few instructions
           if (p.y_pair) {

@@ -484,6 +484,25 @@ def test_lowrank_repeats_bit_for_bit_and_alone(ctx, path):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n,x", [(64, 32, 40, "f32"), (33, 32, 40, "f32"), (33, 32, 160, "bf16"), (64, 256, 256, "f16")])
+def test_lowrank_many_units_repeat(ctx, path, rows, k, n, x):
+    # several short units per SM, so that slots of every ring are used again while their last reader may be late
+    import torch
+    count = 700
+    c = LowRankCase(ctx, [rows] * count, [i % 40 if i % 7 else -1 for i in range(count)], [3 + i % 30 for i in range(40)],
+                    k, n, x=x, w="f16", seed=rows)
+    c.run(ctx)
+    first = c.dy.clone()
+    for _ in range(150):
+        c.dy.fill_(77)
+        torch.cuda.synchronize()
+        c.call(ctx.stream)
+        c.bank.check()
+        assert torch.equal(c.dy, first)
+    c.close()
+
+
+@pytest.mark.gpu
 def test_lowrank_streams_and_graph(ctx, path):
     # two calls at once on two streams with one bank and one plan, then a captured call replayed: first as it was
     # captured, then with other inputs, then with the plan set to another batch (both tile lists change)
