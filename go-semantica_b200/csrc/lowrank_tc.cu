@@ -65,7 +65,7 @@ constexpr int kThreads = (kXWarps + kEpiWarps + 8) * 32;  // the last warpgroups
 // Registers: 1024 threads get 64 each at launch; the last two warpgroups (and
 // the X warps of 16-bit rows, which split nothing) give some back to the
 // epilogue's. The shared memory leaves the L1 too small for spills: with
-// 12 to 60 bytes of them (72, 72 and 40 registers) 102 thousand bf16 rows,
+// 12 to 60 bytes of them (72, 72 and 40 registers) 110213 bf16 rows,
 // 768 x 2304, rank to 64, took 365 us and takes 306 without.
 template <class XT>
 struct Regs {
@@ -501,6 +501,9 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             const uint32_t d = smem_u32(dst) + at0 + i * XR * 128;
             if (ks < full_stages) {
               copy16(d, row[i] + ks * KS, 16);
+            } else if (p.x_four && (ks + 1) * KS <= k) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) copy4(d + j * 4, row[i] + ks * KS + j * (4 / (int)sizeof(XT)), 4);
             } else if (p.x_four) {  // what lies behind k is zeros (that A's are zeros is not enough for a NaN)
               constexpr int E4 = 4 / sizeof(XT);
 #pragma unroll
@@ -632,14 +635,32 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 #pragma unroll
           for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + row_of(j + lane / LPR) * p.a.ldb, bytes);
         } else if (p.b_copy == 4) {
-          constexpr int E4 = 4 / sizeof(YT);
-#pragma unroll 2
-          for (int r = 0; r < B; ++r) {
-            const YT* src = base + row_of(r) * p.a.ldb;
+          constexpr int E4 = 4 / sizeof(YT), NC = 2 / E4;  // copies of a lane per row
+          const YT* col[NC];
+          int bytes[NC];
 #pragma unroll
-            for (int c = lane * E4; c < 64; c += 32 * E4) {
-              const int bytes = max(0, min(4, (in - c) * (int)sizeof(YT)));
-              copy4(fslot + r * RB + c * sizeof(YT), src + (bytes ? ch + c : 0), bytes);
+          for (int q = 0; q < NC; ++q) {
+            const int c = lane * E4 + 32 * q;
+            bytes[q] = max(0, min(4, (in - c) * (int)sizeof(YT)));
+            col[q] = base + (bytes[q] ? ch + c : 0);
+          }
+          const uint32_t dst = fslot + lane * 4;
+          if (frow0 >= 0 && fi + B <= fi1) {  // the usual case in few instructions: they bound unaligned rows
+#pragma unroll
+            for (int q = 0; q < NC; ++q) col[q] += ((int64_t)frow0 + fi - i0) * p.a.ldb;
+#pragma unroll
+            for (int r = 0; r < B; ++r)
+#pragma unroll
+              for (int q = 0; q < NC; ++q) {
+                copy4(dst + r * RB + q * 128, col[q], bytes[q]);
+                col[q] += p.a.ldb;
+              }
+          } else {
+#pragma unroll 2
+            for (int r = 0; r < B; ++r) {
+              const int64_t o = row_of(r) * p.a.ldb;
+#pragma unroll
+              for (int q = 0; q < NC; ++q) copy4(dst + r * RB + q * 128, col[q] + o, bytes[q]);
             }
           }
         } else if constexpr (sizeof(YT) == 2) {  // odd 16-bit addresses: loads, clamped instead of conditional
@@ -759,23 +780,33 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             // single values: exchanged so that the lanes' channels follow each other, lane and lane + 32
             const int c0 = ch - lane;
             auto swap = [&](int from, const Pair& v) -> YT {
-              const uint32_t bits = __shfl_sync(0xffffffffu, raw_bits(v.e[0]), from);
-              const uint32_t odd = __shfl_sync(0xffffffffu, raw_bits(v.e[1]), from);
-              return from_bits<YT>(lane & 1 ? odd : bits);
+              if constexpr (sizeof(YT) == 2) {
+                const uint32_t both = __shfl_sync(0xffffffffu, raw_bits(v.e[0]) | raw_bits(v.e[1]) << 16, from);
+                return from_bits<YT>(lane & 1 ? both >> 16 : both);
+              } else {
+                const uint32_t bits = __shfl_sync(0xffffffffu, raw_bits(v.e[0]), from);
+                const uint32_t odd = __shfl_sync(0xffffffffu, raw_bits(v.e[1]), from);
+                return from_bits<YT>(lane & 1 ? odd : bits);
+              }
             };
-            YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + c0;
+            const bool first = c0 < n_out, second = c0 + 32 < n_out;
+            if (whole) {
+              YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + c0;
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-              const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
-              if (!whole) {
+              for (int j = 0; j < S; ++j, dst += p.a.ldy) {
+                const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
+                if (first) dst[0] = lo;
+                if (second) dst[32] = hi;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < S; ++j) {
+                const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
                 const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
-                dst = y + (int64_t)row * p.a.ldy + c0;
+                YT* dst = y + (int64_t)row * p.a.ldy + c0;
+                if (first && i + j < i1) dst[0] = lo;
+                if (second && i + j < i1) dst[32] = hi;
               }
-              if (i + j < i1) {
-                if (c0 < n_out) dst[0] = lo;
-                if (c0 + 32 < n_out) dst[32] = hi;
-              }
-              dst += p.a.ldy;
             }
           }
         }
