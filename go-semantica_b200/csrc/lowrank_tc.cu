@@ -581,8 +581,17 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
     const uint32_t ring = smem_u32(sE) + (warp - kWarpEpi) * p.epi_ring;
     // this warp's rows [i0, i1) of a unit: a fourth of them, eight at least
     const int per = max(S, p.rt / 4), i0 = ((warp - kWarpEpi) >> 2) * per;
-    // the cursor of the copies: a unit, chunk fc of [.., fc1), rows from fi. The rows follow each other from frow0
-    // (that of row i0), or lane i holds row i0 + i.
+    // Lane i has row i0 + i of the unit, or its group's last one; first_row is that of the group's first lane when its
+    // n rows follow each other (they increase), else -1.
+    auto my_row = [&](const Unit& un, int end) -> int {
+      const int i = min(i0 + lane, end - 1);
+      return un.row0 >= 0 ? un.row0 + i : p.plan.pos_row[un.pos0 + i];
+    };
+    auto first_row = [&](int row, int n) -> int {
+      const int first = __shfl_sync(0xffffffffu, row, 0);
+      return __shfl_sync(0xffffffffu, row, n - 1) - first == n - 1 ? first : -1;
+    };
+    // the cursor of the copies: a unit, chunk fc of [.., fc1), rows from fi; its lane's row and its first row
     UnitCursor fu, uc;
     int fc = 0, fc1 = 0, fi = 0, fi1 = 0, frow0 = 0, frow = 0;
     uint64_t* bars = efull + (warp - kWarpEpi) * 4;
@@ -600,8 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         ++ahead;
         fi1 = min(un.rows, i0 + per);
         if (un.rank == 0 || i0 >= fi1) continue;
-        frow0 = un.row0 < 0 ? -1 : un.row0 + i0;
-        if (frow0 < 0) frow = p.plan.pos_row[un.pos0 + min(i0 + lane, fi1 - 1)];
+        frow = my_row(un, fi1);
+        frow0 = first_row(frow, fi1 - i0);
         fc = un.c0, fc1 = un.c1, fi = i0;
         return true;
       }
@@ -611,10 +620,8 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
       if (!more) more = open();
       if (more) {
         const int ch = fc * 256 + quarter * 64, in = min(64, n_out - ch);  // channels of this warp's there are
-        // rows behind the unit's last one read it again
-        auto row_of = [&](int r) -> int64_t {
-          return frow0 >= 0 ? (int64_t)frow0 + min(fi + r, fi1 - 1) - i0
-                            : (int64_t)__shfl_sync(0xffffffffu, frow, fi - i0 + r);
+        auto off = [&](int r) -> int64_t {  // rows behind the group's last one: that one again
+          return __shfl_sync(0xffffffffu, frow, fi - i0 + r) * p.a.ldb;
         };
         const uint32_t fslot = ring + fr.slot * (B * RB);
         const bool tma = p.b_copy == 16 && frow0 >= 0 && fi + B <= fi1;  // a box holds rows of the unit only
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           const uint32_t dst = fslot + lane / LPR * RB + c * sizeof(YT);
           const YT* col = base + (bytes ? ch + c : 0);
 #pragma unroll
-          for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + row_of(j + lane / LPR) * p.a.ldb, bytes);
+          for (int j = 0; j < B; j += RPI) copy16(dst + j * RB, col + off(j + lane / LPR), bytes);
         } else if (p.b_copy == 4) {
           constexpr int E4 = 4 / sizeof(YT), NC = 2 / E4;  // copies of a lane per row
           const YT* col[NC];
@@ -658,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           } else {
 #pragma unroll 2
             for (int r = 0; r < B; ++r) {
-              const int64_t o = row_of(r) * p.a.ldb;
+              const int64_t o = off(r);
 #pragma unroll
               for (int q = 0; q < NC; ++q) copy4(dst + r * RB + q * 128, col[q] + o, bytes[q]);
             }
@@ -668,15 +675,15 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           const YT* c1 = base + min(ch + lane + 32, n_out - 1);
           YT* dst = reinterpret_cast<YT*>(sE + (fslot - smem_u32(sE)));
 #pragma unroll 1
-          for (int r = 0; r < B; r += 4) {
-            YT v0[4], v1[4];
+          for (int r = 0; r < B; r += 2) {
+            YT v0[2], v1[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int64_t o = row_of(r + j) * p.a.ldb;
+            for (int j = 0; j < 2; ++j) {
+              const int64_t o = off(r + j);
               v0[j] = c0[o], v1[j] = c1[o];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[(r + j) * 64 + lane] = v0[j], dst[(r + j) * 64 + lane + 32] = v1[j];
+            for (int j = 0; j < 2; ++j) dst[(r + j) * 64 + lane] = v0[j], dst[(r + j) * 64 + lane + 32] = v1[j];
           }
         }
         fr.next(nb);
@@ -716,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
         continue;
       }
       const int i1 = min(un.rows, i0 + per);
-      const int my_row = un.row0 < 0 && i0 < i1 ? p.plan.pos_row[un.pos0 + min(i0 + lane, i1 - 1)] : 0;
+      const int row = i0 < i1 ? my_row(un, i1) : 0, row0 = first_row(row, i1 - i0);
       for (int c = un.c0; c < un.c1; ++c, ++d) {
         ok = warp_wait(&dfull[d & 1], (d >> 1) & 1, abort_flag, err, 2u);
         if (!ok) break;
@@ -761,19 +768,19 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             --filled;
             fill();
           }
-          const bool whole = un.row0 >= 0 && i + S <= i1;  // the usual case in few instructions
+          const bool whole = row0 >= 0 && i + S <= i1;  // the usual case in few instructions
           if (p.y_pair) {
             if (whole) {
               if (ch < n_out) {
-                YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + ch;
+                YT* dst = y + (int64_t)(row0 + i - i0) * p.a.ldy + ch;
 #pragma unroll
                 for (int j = 0; j < S; ++j, dst += p.a.ldy) *reinterpret_cast<Pair*>(dst) = b[j];
               }
             } else {
 #pragma unroll
               for (int j = 0; j < S; ++j) {
-                const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
-                if (i + j < i1 && ch < n_out) *reinterpret_cast<Pair*>(y + (int64_t)row * p.a.ldy + ch) = b[j];
+                YT* dst = y + __shfl_sync(0xffffffffu, row, i - i0 + j) * p.a.ldy + ch;
+                if (i + j < i1 && ch < n_out) *reinterpret_cast<Pair*>(dst) = b[j];
               }
             }
           } else {
@@ -791,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
             };
             const bool first = c0 < n_out, second = c0 + 32 < n_out;
             if (whole) {
-              YT* dst = y + (int64_t)(un.row0 + i) * p.a.ldy + c0;
+              YT* dst = y + (int64_t)(row0 + i - i0) * p.a.ldy + c0;
 #pragma unroll
               for (int j = 0; j < S; ++j, dst += p.a.ldy) {
                 const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
@@ -802,8 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 #pragma unroll
               for (int j = 0; j < S; ++j) {
                 const YT lo = swap(lane >> 1, b[j]), hi = swap(16 + (lane >> 1), b[j]);
-                const int row = un.row0 >= 0 ? un.row0 + i + j : __shfl_sync(0xffffffffu, my_row, i - i0 + j);
-                YT* dst = y + (int64_t)row * p.a.ldy + c0;
+                YT* dst = y + __shfl_sync(0xffffffffu, row, i - i0 + j) * p.a.ldy + c0;
                 if (first && i + j < i1) dst[0] = lo;
                 if (second && i + j < i1) dst[32] = hi;
               }
