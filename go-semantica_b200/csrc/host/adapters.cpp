@@ -228,11 +228,11 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, const LowRankArgs& ar
 // Up to this many multiply-adds a call runs on the CUDA cores as a whole: the
 // tensor-core kernel's pipeline takes longer to fill than they take. Measured
 // (CUDA cores / tensor cores, 768 x 768, rank 16): INT8 codes 12.6 M 8.3 / 12.0
-// us, 25 M 12.0 / 13.4, 50 M 18.7 / 14.5; float32 rows, whose conversion the
-// tensor cores wait for, 25 M 11.3 / 19.9; 517 x 1001, 168 M 48.7 / 44.8. A tile
-// of up to 16 rows counts as eight (256 single fp16 rows of as many adapters:
-// 33.3 / 25.0 us; 64 tiles of 12 rows: 13.1 on the CUDA cores).
-constexpr int64_t kLowRankSmallWork = 28000000, kLowRankSmallWorkF32 = 80000000;
+// us, 25 M 12.1 / 13.2, 50 M 18.7 / 14.5; float32 rows, whose conversion the
+// tensor cores wait for, 25 M 11.4 / 19.6, 63 M 21.7 / 21.8; 517 x 1001, 212 M
+// 43.1 / 34.6. A tile of up to 16 rows counts as eight (256 single fp16 rows of
+// as many adapters: 33.3 / 25.0 us; 64 tiles of 12 rows: 13.1 on the CUDA cores).
+constexpr int64_t kLowRankSmallWork = 28000000, kLowRankSmallWorkF32 = 60000000;
 
 // One launch for all tiles of the plan, also for an empty plan when it is
 // captured (a replay may find the plan set to another batch).

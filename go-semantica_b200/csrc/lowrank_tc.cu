@@ -36,15 +36,15 @@
 //     ahead of the accumulators and across units.
 // One persistent CTA per SM. Per call (device time; bytes at 6.56 TB/s, the
 // rate of a plain copy, in parentheses):
-//   65536 float32 rows, 768 x 768, rank 16:             114 us (92)
-//   196608 rows of codes, 1152 x 768, rank 32:          285 us (253)
-//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    314 us (181)
+//   65536 float32 rows, 768 x 768, rank 16:             115 us (92)
+//   196608 rows of codes, 1152 x 768, rank 32:          290 us (253)
+//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    292 us (181)
 //   16384 fp16 rows, 768 x 1280, rank 128, f32 weights:  93 us (17)
-//   6075 ragged float32 rows, 517 x 1001, rank to 23:    45 us (9)
+//   6075 ragged float32 rows, 517 x 1001, rank to 23:    35 us (9)
 // The first two are near the copy's rate. In the third a unit reads 0.6 MB of
 // B from L2 beside its 0.7 MB of rows, in the fourth 1.7 beside 0.4: weights
 // in wide planes for tiles of 64 rows are what larger ranks pay. The last has
-// no TMA for its rows: copies of 4 bytes and single stores.
+// no TMA for its rows: copies of 4 bytes and single stores, in one unit per SM.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -1180,7 +1180,7 @@ cudaError_t tc_types(TcParams p, int n_large, int n_small, cudaStream_t st) {
   p.rt = kRt;
   p.splits = 1;
   // Fewer rows per unit, then shares of the channels, while all units still run at once: a unit's time is mostly its
-  // pipeline's latency (6075 ragged float32 rows, 512 x 1024, rank 23: 36.5 us in one round of 64-row units, 39.6 in
+  // pipeline's latency (6075 ragged float32 rows, 512 x 1024, rank 23: 27.0 us in one round of 64-row units, 29.9 in
   // two rounds of 32).
   auto units = [&](int rt, int splits) { return ((int64_t)n_large * (kAdapterTileRows / rt) + n_small) * splits; };
   while (p.rt > 16 && units(p.rt / 2, 1) <= sms) p.rt /= 2;
