@@ -205,7 +205,6 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
     }
     __syncthreads();
     float* part = s_part + set * kSmallParts * kSmallRows * bank.max_rank;
-    set ^= 1;
     const int size = ad.rank * kSmallRows;
     // a thread: four rows of a pair of output channels; base and the first ranks of B are on their way while t is summed
     const int items = (n1 - n0 + 1) / 2 * (kSmallRows / 4);
@@ -282,6 +281,10 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
     }
     if (ad.rank > 0) {
       cluster.sync();
+      // The sets of partials take turns over the units that have this barrier: a set is written again only behind the
+      // next such unit's barrier, which every CTA reaches with its sums below done. (A unit of rank 0 must not count:
+      // the third unit's partials would land in a set that a slower CTA still sums.)
+      set ^= 1;
       for (int i = tid; i < ad.rp * kSmallRows; i += kSmallThreads) {
         float v = 0.0f;
         if (i < size) {
