@@ -209,12 +209,19 @@ int lowrank_create(sem_context* ctx, int32_t k_in, int32_t n_out, int32_t n_adap
 
 namespace {
 
-// The checks that both forms of the call share; *st receives the stream.
-int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, const LowRankArgs& args, void* stream) {
+// What both forms of the call share. The plan is looked at and the call enqueued under one lock, so that the batch
+// that the checks saw is the one that the call runs on. n_absmax: the activation scales given (null: none).
+int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, LowRankArgs args, const int32_t* n_absmax, void* stream) {
   if (int rc = same_device(w->ctx, plan->ctx)) return rc;
   DeviceGuard dg(w->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : w->ctx->stream;
   std::lock_guard<std::mutex> lk(plan->mu);
+  if (n_absmax) {
+    if (*n_absmax != 1 && *n_absmax != plan->n_seqs)
+      return set_error(SEM_EINVAL, "low-rank adapters: %d activation scales for a plan of %d sequences", *n_absmax,
+                       plan->n_seqs);
+    args.per_seq = *n_absmax != 1;
+  }
   if (plan->max_adapter >= w->bank.n_adapters)
     return set_error(SEM_EINVAL, "low-rank adapters: the plan uses adapter %d, the bank has %d", plan->max_adapter,
                      w->bank.n_adapters);
@@ -276,7 +283,7 @@ int lowrank_apply(sem_lowrank* w, sem_adapter_plan* plan, const void* d_x, int32
   if (d_base == d_y && ld_base != ldy)
     return set_error(SEM_EINVAL, "low-rank adapters: base and outputs are one buffer with two row strides");
   LowRankArgs a{d_x, d_base, d_y, ldx, ld_base, ldy, x_dtype, y_dtype, nullptr, 0};
-  return lowrank_launch(w, plan, a, stream);
+  return lowrank_launch(w, plan, a, nullptr, stream);
 }
 
 int lowrank_apply_int8(sem_lowrank* w, sem_adapter_plan* plan, const void* d_codes, const uint32_t* d_absmax,
@@ -291,15 +298,8 @@ int lowrank_apply_int8(sem_lowrank* w, sem_adapter_plan* plan, const void* d_cod
     return set_error(SEM_EINVAL, "low-rank adapters: a pointer is not aligned to its element type");
   if (d_base == d_y && ld_base != ldy)
     return set_error(SEM_EINVAL, "low-rank adapters: base and outputs are one buffer with two row strides");
-  {
-    std::lock_guard<std::mutex> lk(plan->mu);
-    if (n_absmax != 1 && n_absmax != plan->n_seqs)
-      return set_error(SEM_EINVAL, "low-rank adapters: %d activation scales for a plan of %d sequences", n_absmax,
-                       plan->n_seqs);
-  }
-  LowRankArgs a{d_codes, d_base, d_y, w->bank.k_in, ld_base, ldy, SEM_DTYPE_F16, SEM_DTYPE_F32, d_absmax,
-                n_absmax != 1};
-  return lowrank_launch(w, plan, a, stream);
+  LowRankArgs a{d_codes, d_base, d_y, w->bank.k_in, ld_base, ldy, SEM_DTYPE_F16, SEM_DTYPE_F32, d_absmax, 0};
+  return lowrank_launch(w, plan, a, &n_absmax, stream);
 }
 
 int lowrank_check(sem_lowrank* w) {
@@ -393,9 +393,10 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
     return set_error(SEM_EINVAL, "block norm: one buffer with two row strides");
   DeviceGuard dg(b->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : b->ctx->stream;
+  std::unique_lock<std::mutex> lk;  // until the call is enqueued, as in lowrank_launch
   if (plan) {
     if ((rc = same_device(b->ctx, plan->ctx))) return rc;
-    std::lock_guard<std::mutex> lk(plan->mu);
+    lk = std::unique_lock<std::mutex>(plan->mu);
     if (plan->rows != rows)
       return set_error(SEM_EINVAL, "block norm: %lld rows, the plan has %d", (long long)rows, plan->rows);
     if ((b->gates || b->scales) && plan->max_adapter >= b->n_adapters)

@@ -67,3 +67,90 @@ def test_one_cluster_takes_many_units_with_and_without_rank(ctx, captured, x):
     finally:
         lib.sem_lowrank_path(prev)
     c.close()
+
+
+@pytest.mark.gpu
+def test_int8_scales_are_checked_against_the_batch_they_meet(ctx):
+    # One thread sets the plan to a batch of two sequences and to one of sixteen in turn, another calls with two
+    # scales: a call is refused, or it runs on the batch of two. The scales behind the second one are NaN, which
+    # would stay in y (a sum in place) for good.
+    import _lib
+    import torch
+    import adapters as ad
+    k, n, rows = 32, 32, 32
+    rng = np.random.default_rng(0)
+    bank = ad.LowRank(ctx, k, n, [rng.standard_normal((2, k)).astype(np.float32)],
+                      [rng.standard_normal((n, 2)).astype(np.float32)], [1e-6], ad.F32)
+    plan = ad.AdapterPlan(ctx, rows, 16)
+    two, sixteen = ([0, 16, 32], [0, 0]), (list(range(0, 33, 2)), [0] * 16)
+    codes = torch.randint(-127, 128, (rows, k), device="cuda").half()
+    absmax = torch.full((16,), float("nan"), device="cuda")
+    absmax[:2] = 1.0
+    y = torch.zeros(rows, n, device="cuda")
+    torch.cuda.synchronize()
+    plan.set(*sixteen)
+    done, took = threading.Event(), [0, 0]
+
+    def setter():
+        while not done.is_set():
+            plan.set(*two)
+            plan.set(*sixteen)
+
+    def caller():
+        try:
+            for _ in range(20000):
+                try:
+                    bank.apply_int8(plan, codes.data_ptr(), absmax.data_ptr(), 2, y.data_ptr(), y.data_ptr())
+                    took[0] += 1
+                except _lib.SemError as e:
+                    assert "2 activation scales for a plan of 16 sequences" in str(e)
+                    took[1] += 1
+        finally:
+            done.set()
+
+    _threads(setter, caller)
+    bank.check()
+    assert took[0] and took[1], took  # both batches were met
+    assert torch.isfinite(y).all(), torch.isfinite(y).all(1)
+    bank.close()
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_block_norm_runs_on_the_batch_it_was_checked_against(ctx):
+    # The plan is set to 40 rows without an adapter and to 20 of adapter 0 in turn: a call over 40 rows is refused or
+    # runs on the first. Adapter 0's gate is NaN, which would stay in the residual stream (in place) for good.
+    import _lib
+    import torch
+    import adapters as ad
+    dim, rows = 64, 40
+    bn = ad.BlockNorm(ctx, dim, 1e-6, gates=np.full((1, dim), np.nan, np.float32))
+    plan = ad.AdapterPlan(ctx, rows, 1)
+    o, h = torch.zeros(rows, dim, device="cuda"), torch.ones(rows, dim, device="cuda")
+    torch.cuda.synchronize()
+    plan.set([0, 20], [0])
+    done, took = threading.Event(), [0, 0]
+
+    def setter():
+        while not done.is_set():
+            plan.set([0, 40], [-1])
+            plan.set([0, 20], [0])
+
+    def caller():
+        try:
+            for _ in range(20000):
+                try:
+                    bn.run(rows, o.data_ptr(), 0, h.data_ptr(), 0, h.data_ptr(), plan=plan)
+                    took[0] += 1
+                except _lib.SemError as e:
+                    assert "40 rows, the plan has 20" in str(e)
+                    took[1] += 1
+        finally:
+            done.set()
+
+    _threads(setter, caller)
+    torch.cuda.synchronize()
+    assert took[0] and took[1], took
+    assert (h == 1).all()
+    bn.close()
+    plan.close()
