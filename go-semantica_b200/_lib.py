@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "libsemantica_b200.so")
 SEM_OK, SEM_EINVAL, SEM_EDEVICE, SEM_ENOMEM, SEM_EFORMAT, SEM_ENOTFOUND, SEM_EINTERNAL = range(7)
 SEARCH_REFERENCE, SEARCH_EXACT = 0, 1
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = range(3)
+ABSMAX_ALL_ROWS, ABSMAX_PER_SEQUENCE = -2, -3
 
 
 class SemError(Exception):

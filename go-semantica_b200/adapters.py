@@ -13,6 +13,7 @@ import ctypes as C
 
 import numpy as np
 
+from _lib import ABSMAX_ALL_ROWS, ABSMAX_PER_SEQUENCE
 from _lib import DTYPE_BF16 as BF16
 from _lib import DTYPE_F16 as F16
 from _lib import DTYPE_F32 as F32
@@ -107,7 +108,8 @@ class LowRank(_Handle):
 
     def apply_int8(self, plan: AdapterPlan, d_codes: int, d_absmax: int, n_absmax: int, d_y: int, d_base: int = 0,
                    ld_base: int = 0, ldy: int = 0, stream: int = 0) -> None:
-        """The same on INT8 codes held as fp16 with one activation scale, or one per sequence."""
+        """The same on INT8 codes held as fp16 with one activation scale (n_absmax 1 or ABSMAX_ALL_ROWS), or one per
+        sequence (their number or ABSMAX_PER_SEQUENCE; by name in a capture on a plan of one sequence)."""
         check(load().sem_lowrank_apply_int8(self.handle, plan.handle, d_codes, d_absmax, n_absmax, d_base or None,
                                             ld_base, d_y, ldy, stream or None))
 
@@ -147,4 +149,4 @@ class BlockNorm(_Handle):
                                         d_h, ldh, h_dtype, d_h_out, ld_h_out, d_y or None, ldy, stream or None))
 
 
-__all__ = ["AdapterPlan", "LowRank", "BlockNorm", "F32", "F16", "BF16"]
+__all__ = ["AdapterPlan", "LowRank", "BlockNorm", "F32", "F16", "BF16", "ABSMAX_ALL_ROWS", "ABSMAX_PER_SEQUENCE"]

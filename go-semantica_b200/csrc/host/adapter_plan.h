@@ -7,6 +7,8 @@
 #include <cstdint>
 #include <vector>
 
+#include "../../../include/semantica_b200.h"
+
 namespace sem {
 
 // Rows of a large tile, and the most rows of a small one (the kernels of
@@ -52,6 +54,20 @@ inline const char* adapter_plan_check(const int32_t* offsets, const int32_t* ada
   }
   *bad = -1;
   if (n_seqs > 0 && offsets[n_seqs] > max_rows) return "more rows than the plan was created for";
+  return nullptr;
+}
+
+// What n_absmax activation scales of a call belong to: *per_seq 1, one per
+// sequence of a plan of n_seqs; 0, one for every row. A capture keeps the
+// answer for batches of other counts, so there the count has to tell the two
+// apart. Returns why not, nullptr when it does.
+inline const char* lowrank_scales(int32_t n_absmax, int32_t n_seqs, bool captured, int32_t* per_seq) {
+  *per_seq = n_absmax == SEM_ABSMAX_PER_SEQUENCE || (n_absmax != 1 && n_absmax == n_seqs);
+  if (*per_seq || n_absmax == SEM_ABSMAX_ALL_ROWS) return nullptr;
+  if (n_absmax != 1) return "neither one for all rows nor one per sequence";
+  if (captured && n_seqs == 1)
+    return "a call captured with 1 activation scale for a plan of 1 sequence has to say SEM_ABSMAX_ALL_ROWS or "
+           "SEM_ABSMAX_PER_SEQUENCE";
   return nullptr;
 }
 

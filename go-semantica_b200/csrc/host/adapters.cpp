@@ -216,17 +216,15 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, LowRankArgs args, con
   DeviceGuard dg(w->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : w->ctx->stream;
   std::lock_guard<std::mutex> lk(plan->mu);
-  if (n_absmax) {
-    if (*n_absmax != 1 && *n_absmax != plan->n_seqs)
-      return set_error(SEM_EINVAL, "low-rank adapters: %d activation scales for a plan of %d sequences", *n_absmax,
-                       plan->n_seqs);
-    args.per_seq = *n_absmax != 1;
-  }
   if (plan->max_adapter >= w->bank.n_adapters)
     return set_error(SEM_EINVAL, "low-rank adapters: the plan uses adapter %d, the bank has %d", plan->max_adapter,
                      w->bank.n_adapters);
   bool cap = false;
   if (int rc = capturing(st, &cap)) return rc;
+  if (n_absmax)
+    if (const char* why = lowrank_scales(*n_absmax, plan->n_seqs, cap, &args.per_seq))
+      return set_error(SEM_EINVAL, "low-rank adapters: %d activation scales for a plan of %d sequences: %s", *n_absmax,
+                       plan->n_seqs, why);
   return lowrank_enqueue(w->bank, plan, args, cap, w->err.as<uint32_t>(), st);
 }
 

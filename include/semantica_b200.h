@@ -346,8 +346,15 @@ int sem_lowrank_apply(sem_lowrank *w, sem_adapter_plan *plan, const void *d_x, i
                       const void *d_base, int64_t ld_base, void *d_y, int32_t y_dtype, int64_t ldy, void *stream);
 /* The same beside sem_q8_matmul_int8: x = code * (absmax / 127), d_codes the
  * rows x k_in INT8 codes as fp16, d_absmax the float32 bit patterns of the
- * absmax they were quantised with: one for every row (n_absmax = 1), or one
- * per sequence of the plan (n_absmax = n_seqs). */
+ * absmax they were quantised with. n_absmax says how many and what they
+ * belong to: 1, one for every row; n_seqs, one per sequence of the plan; or
+ * by name, SEM_ABSMAX_ALL_ROWS and SEM_ABSMAX_PER_SEQUENCE, whatever the
+ * plan's batch. A captured call keeps the meaning that it was captured with.
+ * Where a capture meets a plan of one sequence, n_absmax = 1 could be either,
+ * and is refused: name it (a replay may find another batch, for which
+ * d_absmax then has to hold a scale per sequence, or one). */
+#define SEM_ABSMAX_ALL_ROWS (-2)
+#define SEM_ABSMAX_PER_SEQUENCE (-3)
 int sem_lowrank_apply_int8(sem_lowrank *w, sem_adapter_plan *plan, const void *d_codes, const uint32_t *d_absmax,
                            int32_t n_absmax, const float *d_base, int64_t ld_base, float *d_y, int64_t ldy,
                            void *stream);

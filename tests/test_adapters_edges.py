@@ -1,12 +1,16 @@
 """The adapter operators where calls meet one another or the edges of their
 types: captures on one batch replayed on another, calls from several threads,
 infinities, the bits of rows without an adapter."""
+import ctypes as C
+import os
+import subprocess
 import threading
 
 import numpy as np
 import pytest
 
-from test_adapters import DT, LowRankCase, _batch, path  # noqa: F401 (a fixture)
+from conftest import ROOT
+from test_adapters import BUILD, DT, LowRankCase, _batch, path  # noqa: F401 (a fixture)
 
 
 def _threads(*work):
@@ -154,3 +158,90 @@ def test_block_norm_runs_on_the_batch_it_was_checked_against(ctx):
     assert (h == 1).all()
     bn.close()
     plan.close()
+
+
+@pytest.fixture(scope="module")
+def scales_host():
+    os.makedirs(BUILD, exist_ok=True)
+    so = os.path.join(BUILD, "libscales_host.so")
+    r = subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Werror",
+                        os.path.join(ROOT, "tests", "adapters", "scales_host.cpp"), "-o", so],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    lib = C.CDLL(so)
+    lib.sh_scales.restype = C.c_char_p
+    return lib
+
+
+@pytest.mark.parametrize("n_absmax,n_seqs,captured,want", [
+    (1, 1, False, 0), (1, 3, False, 0), (1, 0, False, 0), (3, 3, False, 1), (0, 0, False, 1),
+    (1, 1, True, None), (1, 3, True, 0), (1, 0, True, 0), (3, 3, True, 1), (0, 0, True, 1),
+    (-2, 1, True, 0), (-3, 1, True, 1), (-2, 5, False, 0), (-3, 5, True, 1), (-3, 0, True, 1),
+    (0, 2, False, None), (3, 2, True, None), (2, 1, False, None), (-1, 2, False, None), (-1, 0, False, None),
+])
+def test_what_the_scales_belong_to(scales_host, n_absmax, n_seqs, captured, want):
+    per_seq = C.c_int32(-7)
+    why = scales_host.sh_scales(n_absmax, n_seqs, int(captured), C.byref(per_seq))
+    assert (why == b"") == (want is not None)
+    if want is not None:
+        assert per_seq.value == want
+
+
+def _captured(torch, c, call):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(torch.cuda.current_stream().cuda_stream)
+    return graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", [0, 1, 3])
+def test_captured_int8_call_keeps_its_scales_meaning(ctx, path, start):
+    # captured on an empty batch, on one sequence or on three, replayed on batches of one, three and five
+    import torch
+    c = LowRankCase(ctx, [40, 3, 60, 20, 77], [0, 1, 0, -1, 1], [16, 8], 96, 160, x="f16", y="f32", codes=2)
+    every = c.absmax.clone()
+    batches = {0: ([], []), 1: ([90], [1]), 3: ([40, 3, 60], [0, 1, 0]), 5: ([40, 3, 60, 20, 77], [0, 1, 0, -1, 1])}
+
+    def put(count):
+        lengths, use = batches[count]
+        c.offs, c.use = _batch(lengths, use)
+        c.plan.set(c.offs, c.use)
+        torch.cuda.synchronize()
+
+    put(start)
+    import adapters as ad
+    for mode in (ad.ABSMAX_PER_SEQUENCE, ad.ABSMAX_ALL_ROWS):
+        put(start)
+        graph = _captured(torch, c, lambda st: c.bank.apply_int8(  # noqa: B023
+            c.plan, c.dx.data_ptr(), c.dabs.data_ptr(), mode, c.dy.data_ptr(), c.dbase.data_ptr(), stream=st))  # noqa: B023
+        for count in (1, 3, 5, 3):
+            put(count)
+            c.dy.fill_(77)
+            graph.replay()
+            c.bank.check()
+            lengths, use = batches[count]
+            rows = sum(lengths)
+            c.seq = np.concatenate([np.repeat(np.arange(count), lengths), np.zeros(c.rows - rows, int)])
+            c.adapter = np.concatenate([np.repeat(use, lengths), np.full(c.rows - rows, -1)])
+            c.absmax = every if mode == ad.ABSMAX_PER_SEQUENCE else every[:1]
+            c.codes = 2 if mode == ad.ABSMAX_PER_SEQUENCE else 1
+            want, bound = c.oracle()
+            assert ((c.dy[:rows].cpu().double() - want[:rows]).abs() <= bound[:rows]).all()
+            assert (c.dy[rows:] == 77).all()
+    c.close()
+
+
+@pytest.mark.gpu
+def test_one_scale_for_one_sequence_is_not_captured(ctx):
+    # one number that says both "one for all rows" and "one per sequence": fine for a call, refused in a capture
+    import _lib
+    import torch
+    c = LowRankCase(ctx, [40], [0], [16], 96, 160, x="f16", y="f32", codes=2)
+    c.run(ctx)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        c.dy.fill_(77)
+        with pytest.raises(_lib.SemError, match="captured with 1 activation scale for a plan of 1 sequence"):
+            c.call(torch.cuda.current_stream().cuda_stream)
+    c.run(ctx)
+    c.close()
