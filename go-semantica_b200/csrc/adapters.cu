@@ -512,11 +512,13 @@ template <class XT, class YT, class WT, int RU>
 cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int n_units,
                         const LowRankArgs& a, cudaStream_t st) {
   const int smem = small_smem_floats(bank.max_rank) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-  }
+  // The function's limit is set to the same value whatever the bank (its largest rank's need): another thread may set
+  // it between this call's setting and its launch.
+  constexpr int kMostRank = RU * kSmallWarps;
+  const cudaError_t e =
+      cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           small_smem_floats(kMostRank) * 4);
+  if (e != cudaSuccess) return e;
   // the largest clusters whose CTAs are all on the device at once (three per SM, two at ranks above 32; 132 SMs, since
   // a cluster of eight leaves some of a processing cluster's unused): 64 units of rank 16 took 20.5 us on clusters of
   // eight, in two waves, and take 13.1 us on clusters of four

@@ -245,3 +245,41 @@ def test_one_scale_for_one_sequence_is_not_captured(ctx):
             c.call(torch.cuda.current_stream().cuda_stream)
     c.run(ctx)
     c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ranks", [(128, 40), (32, 27)])
+def test_banks_of_other_ranks_at_the_same_time(ctx, ranks):
+    # two threads, each with a bank, a plan and a stream of its own, on the CUDA cores: their kernels are one function
+    # with different needs of shared memory
+    import _lib
+    import torch
+    so = os.path.join(BUILD, "libcalls.so")
+    os.makedirs(BUILD, exist_ok=True)
+    r = subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-Wall", "-Werror",
+                        os.path.join(ROOT, "tests", "adapters", "calls.cpp"), "-o", so], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    repeat = C.CDLL(so).repeat_apply
+    repeat.argtypes = [C.c_void_p] * 7 + [C.c_int32]
+    lib = _lib.load()
+    prev = lib.sem_lowrank_path(1)
+    cases = [LowRankCase(ctx, [3, 9], [0, -1], [r], 64, 64, seed=r) for r in ranks]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    failed = [None, None]
+
+    def caller(i):
+        c = cases[i]
+        failed[i] = repeat(C.cast(lib.sem_lowrank_apply, C.c_void_p), c.bank.handle, c.plan.handle, c.dx.data_ptr(),
+                           c.dbase.data_ptr(), c.dy.data_ptr(), streams[i].cuda_stream, 50000)
+
+    try:
+        _threads(lambda: caller(0), lambda: caller(1))
+        assert failed == [0, 0]
+        for c in cases:
+            c.bank.check()
+            c.verify(c.dy)
+    finally:
+        lib.sem_lowrank_path(prev)
+    for c in cases:
+        c.close()
