@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
       for (int i = 0; i < 4; ++i) {
         if (q * 4 + i >= rows) break;
         YT* d = y + (int64_t)s_row[q * 4 + i] * a.ldy + ch;
-        d[0] = from_f32<YT>(__fadd_rn(to_f32(b[0][i]), o[0][i]));
-        if (ch + 1 < n1) d[1] = from_f32<YT>(__fadd_rn(to_f32(b[1][i]), o[1][i]));
+        // without a rank base as it is: adding a zero would change the sign of a zero and the bits of a NaN
+        d[0] = ad.rank > 0 ? from_f32<YT>(__fadd_rn(to_f32(b[0][i]), o[0][i])) : b[0][i];
+        if (ch + 1 < n1) d[1] = ad.rank > 0 ? from_f32<YT>(__fadd_rn(to_f32(b[1][i]), o[1][i])) : b[1][i];
       }
     }
   }

@@ -283,3 +283,26 @@ def test_banks_of_other_ranks_at_the_same_time(ctx, ranks):
         lib.sem_lowrank_path(prev)
     for c in cases:
         c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,y", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_rows_without_an_adapter_keep_their_bits(ctx, path, x, y):
+    # y = base for them: the sign of a zero and the bits of a NaN too
+    import torch
+    c = LowRankCase(ctx, [5, 20, 70, 3], [-1, 1, 0, 2], [0, 16, 4], 64, 96, x=x, y=y)
+    word = torch.int32 if y == "f32" else torch.int16
+    nan = torch.tensor([{"f32": 0x7fc12345, "f16": 0x7e45, "bf16": 0x7fc5}[y]], dtype=word).view(c.base.dtype)
+    plain = torch.from_numpy(~np.isin(c.adapter, [1, 2]))
+    assert plain.any() and not plain.all()
+    c.base[plain, 1::3] = -0.0
+    c.base[plain, 2::3] = nan
+    c.dbase.copy_(c.base)
+    torch.cuda.synchronize()
+    c.call(ctx.stream)
+    c.bank.check()
+    got = c.dy.cpu()
+    assert torch.equal(got[plain].view(word), c.base[plain].view(word))
+    want, bound = c.oracle()
+    assert ((got[~plain].double() - want[~plain]).abs() <= bound[~plain]).all()
+    c.close()
