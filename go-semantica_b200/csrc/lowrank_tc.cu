@@ -187,13 +187,18 @@ __device__ __forceinline__ void copy_wait(int n) {
   }
 }
 
-// v = hi + lo: hi the upper 11 significant bits. |lo| < 2^-11 * 2^128 < 2e35,
-// so the maximum only replaces the NaN that an infinite v leaves in lo (which
-// would turn an infinite result into NaN); a NaN v stays one in hi. lo's bits
-// behind its own 11 are cut too: an operand is a tf32 value.
+// v = hi + lo: hi the upper 11 significant bits; lo's bits behind its own 11
+// are cut too: an operand is a tf32 value. An infinite v is hi, and NaN in lo.
+// (The sum makes a NaN a quiet one, which the cut cannot turn into an infinity.)
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
+  v = __fadd_rn(v, 0.0f);
   hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
-  lo = __uint_as_float(__float_as_uint(fmaxf(__fsub_rn(v, hi), -2e35f)) & 0xffffe000u);
+  lo = __uint_as_float(__float_as_uint(__fsub_rn(v, hi)) & 0xffffe000u);
+}
+// The same with lo = 0 for an infinite v (and a NaN).
+__device__ __forceinline__ void split_tf32_lo_finite(float v, float& hi, float& lo) {
+  split_tf32(v, hi, lo);
+  lo = lo == lo ? lo : 0.0f;
 }
 
 template <class T>
@@ -857,13 +862,24 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = __uint_as_float(v[e]);
           }
-          for (int k = 1; k < sa.parts; ++k) {
+          for (int k = 1; k < sa.hi_parts; ++k) {
             uint32_t v[8];
             tmem_ld8(acc + (uint32_t)(k * sa.width + j), v);
             tmem_wait_ld();
             reg_barrier8(v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = __fadd_rn(t[e], __uint_as_float(v[e]));
+          }
+          // The low parts. Where the sum so far is an infinity or NaN it is the result, since every factor is in it with
+          // its sign: an infinity times a low part of zero is a NaN that the formula does not have.
+          if (PX == 2 || PA > 1) {
+            uint32_t v[8];
+            tmem_ld8(acc + (uint32_t)(sa.hi_parts * sa.width + j), v);
+            tmem_wait_ld();
+            reg_barrier8(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (fabsf(t[e]) < __uint_as_float(0x7f800000u)) t[e] = __fadd_rn(t[e], __uint_as_float(v[e]));
           }
           if (XTYPE == kDtF16 && un.unscale) {
 #pragma unroll
@@ -872,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1) lowrank_tc_kernel(const __grid_co
           float hi[8], lo[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)  // ranks behind the last one meet zero columns of B: they have to be finite
-            split_tf32(j + e < un.rank ? __fmul_rn(t[e], sc) : 0.0f, hi[e], lo[e]);
+            split_tf32_lo_finite(j + e < un.rank ? __fmul_rn(t[e], sc) : 0.0f, hi[e], lo[e]);
           uint8_t* dst = sT + tr.slot * t_buf + (j / KC) * 2 * t_plane + row * 128;
           if (row >= p.rt) continue;  // lanes without a row of t (units of 16 rows)
           const int c0 = (j % KC) / 4, x = row & 7;
@@ -1117,7 +1133,10 @@ __global__ void lowrank_tiles_kernel(const LowRankAdapter* ads, int k_in, int n_
     float* dst = reinterpret_cast<float*>(tile + (int64_t)row * 128 + (((c >> 2) ^ (row & 7)) * 16) + (c & 3) * 4);
     if (planes == 2) {
       float hi, lo;
-      split_tf32(v, hi, lo);
+      split_tf32_lo_finite(v, hi, lo);
+      // An infinite t times a low part of zero would be NaN: B's are at least 2^-126, with the weight's sign, where that
+      // is nothing to the weight (A's low products have an accumulator that an infinite sum leaves out).
+      if (i >= na && lo == 0.0f && fabsf(v) >= ldexpf(1.0f, -100)) lo = copysignf(ldexpf(1.0f, -126), v);
       dst[0] = hi;
       dst[plane / 4] = lo;
     } else {

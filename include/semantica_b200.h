@@ -341,7 +341,9 @@ int sem_lowrank_free(sem_lowrank *w);
  * allowed (rows that start on 16 bytes load fastest). Types: x F32 with y
  * F32; x F16 or BF16 with y of the same type or F32. Products and sums are
  * held in float32, with x, the weights and the rank-wide intermediate carried
- * to at least 21 bits; the result is rounded once, to y's type. */
+ * to at least 21 bits; the result is rounded once, to y's type. Infinities and
+ * NaN in x give what the formula gives and stay in their rows (the weights are
+ * finite). */
 int sem_lowrank_apply(sem_lowrank *w, sem_adapter_plan *plan, const void *d_x, int32_t x_dtype, int64_t ldx,
                       const void *d_base, int64_t ld_base, void *d_y, int32_t y_dtype, int64_t ldy, void *stream);
 /* The same beside sem_q8_matmul_int8: x = code * (absmax / 127), d_codes the

@@ -306,3 +306,69 @@ def test_rows_without_an_adapter_keep_their_bits(ctx, path, x, y):
     want, bound = c.oracle()
     assert ((got[~plain].double() - want[~plain]).abs() <= bound[~plain]).all()
     c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,y", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("w", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("short", [False, True])
+def test_infinite_rows_give_the_formulas_infinities(ctx, path, x, y, w, short):
+    # Rank 1 and one infinity in a row of x: every result of the row is infinite, with the formula's sign (no weight is
+    # zero). Rank 3 with weights whose terms agree in sign the same; one infinity of each sign: NaN. `short`: float32
+    # weights whose low parts are all zero.
+    import torch
+    import adapters as ad
+    k, n = 70, 90
+    c = LowRankCase(ctx, [40, 30], [0, 1], [1, 3], k, n, x=x, y=y, w=w, seed=5, scales=[-1.5, 2.0])
+    inf = float("inf")
+
+    def away(t):  # away from zero; of few bits with `short`
+        t = t.float().sign() * (t.float().abs() + 0.01)
+        return (t.to(torch.bfloat16) if short else t).to(t.dtype)
+
+    c.a = [away(t).to(t.dtype) for t in c.a]
+    c.b = [away(t).to(t.dtype) for t in c.b]
+    c.a[1], c.b[1] = c.a[1].abs(), c.b[1].abs()
+    host = lambda t: (t.view(torch.int16) if t.dtype == torch.bfloat16 else t).numpy()  # noqa: E731
+    c.bank.close()
+    c.bank = ad.LowRank(ctx, k, n, [host(t) for t in c.a], [host(t) for t in c.b], c.scales, DT[w])
+    rows = {0: (3, inf), 7: (69, -inf), 20: (0, inf), 39: (64, -inf), 41: (5, inf), 50: (69, -inf), 69: (33, inf)}
+    for r, (col, v) in rows.items():
+        c.x[r, col] = v
+    c.x[60, 2], c.x[60, 8] = inf, -inf
+    c.dx.copy_(c.x)
+    torch.cuda.synchronize()
+    c.call(ctx.stream)
+    c.bank.check()
+    got = c.dy.cpu().double()
+    for r, (col, v) in rows.items():
+        i = int(c.adapter[r])
+        t = torch.sign(c.a[i][:, col].double()) * v
+        want = c.scales[i] * c.b[i].double() @ t
+        assert torch.isinf(want).all()
+        assert torch.equal(got[r], want), (r, got[r][:8], want[:8])
+    assert torch.isnan(got[60]).all()
+    finite = [r for r in range(c.rows) if r not in rows and r != 60]
+    c.x[list(rows) + [60]] = 0
+    want, bound = c.oracle()
+    assert ((got[finite] - want[finite]).abs() <= bound[finite]).all()
+    c.close()
+
+
+@pytest.mark.gpu
+def test_a_nan_of_any_payload_stays_one(ctx, path):
+    # float32 rows are cut to 11 bits for the tensor cores: a NaN whose payload lies behind them is no infinity
+    import torch
+    c = LowRankCase(ctx, [64, 9], [0, 1], [1, 5], 64, 40, w="f32")
+    bits = c.dx.view(torch.int32)
+    bits[3, 7], bits[60, 63], bits[70, 0] = 0x7f800001, -0x7fffff, 0x7fc00000  # the second: a negative one
+    assert torch.isnan(c.dx).sum() == 3
+    torch.cuda.synchronize()
+    c.call(ctx.stream)
+    c.bank.check()
+    got, bad = c.dy.cpu(), [3, 60, 70]
+    assert torch.isnan(got[bad]).all()
+    want, bound = c.oracle()
+    rest = [i for i in range(73) if i not in bad]
+    assert ((got[rest].double() - want[rest]).abs() <= bound[rest]).all()
+    c.close()
