@@ -128,7 +128,7 @@ constexpr int kSmallChunk = 128, kSmallLd = kSmallChunk + 4;  // input channels 
 constexpr int kSmallRows = kAdapterSmallRows;
 static_assert(kSmallRows == 16, "a thread's row is its lane modulo 16");
 
-inline __host__ __device__ int small_smem_floats(int max_rank) {  // x, A, the partials of two units in turn, t
+inline __host__ __device__ constexpr int small_smem_floats(int max_rank) {  // x, A, the partials of two units in turn, t
   return (kSmallRows + max_rank) * kSmallLd + 2 * kSmallParts * kSmallRows * max_rank + kSmallRows * ((max_rank + 7) & ~7);
 }
 
@@ -204,6 +204,20 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
       s_scale[tid] = sc;
     }
     __syncthreads();
+    if (ad.rank == 0) {  // base as it is: adding a zero would change the sign of a zero and the bits of a NaN
+      for (int r = warp; r < rows; r += kSmallWarps) {
+        const int64_t row = s_row[r];
+        for (int c = n0 + lane; c < n1; c += 128) {  // four loads in flight
+          YT v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = base ? base[row * a.ldb + min(c + 32 * i, n1 - 1)] : from_f32<YT>(0.0f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + 32 * i < n1) y[row * a.ldy + c + 32 * i] = v[i];
+        }
+      }
+      continue;  // the whole cluster
+    }
     float* part = s_part + set * kSmallParts * kSmallRows * bank.max_rank;
     const int size = ad.rank * kSmallRows;
     // a thread: four rows of a pair of output channels; base and the first ranks of B are on their way while t is summed
@@ -219,83 +233,79 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           b[e][i] = base ? base[(int64_t)s_row[q * 4 + i] * a.ldb + c] : from_f32<YT>(0.0f);
-        if (ad.rank > 0) fetch_weights8(ad.b, (int64_t)c * ad.rp, w[e]);
+        fetch_weights8(ad.b, (int64_t)c * ad.rp, w[e]);
       }
     };
     if (tid < items) fetch(tid);
-    if (ad.rank > 0) {
-      // a thread: one row (lane % 16), half of each chunk's channels (lane / 16), every eighth rank
-      for (int eighth = cta; eighth < kSmallParts; eighth += ctas) {
-        const int k0 = min(bank.k_in, eighth * kper), k1 = min(bank.k_in, k0 + kper);
-        float acc[RU];
+    // a thread: one row (lane % 16), half of each chunk's channels (lane / 16), every eighth rank
+    for (int eighth = cta; eighth < kSmallParts; eighth += ctas) {
+      const int k0 = min(bank.k_in, eighth * kper), k1 = min(bank.k_in, k0 + kper);
+      float acc[RU];
 #pragma unroll
-        for (int i = 0; i < RU; ++i) acc[i] = 0.0f;
-        for (int kc = k0; kc < k1; kc += kSmallChunk) {
-          const int kn = min(kSmallChunk, k1 - kc), oct = (kn + 7) / 8;
-          if (eighth != cta || kc > k0) __syncthreads();
-          auto put = [&](int r, int c, const float (&v)[8]) {
-            float4* d = reinterpret_cast<float4*>(s_x + r * kSmallLd + c);
-            d[0] = make_float4(v[0], v[1], v[2], v[3]);
-            d[1] = make_float4(v[4], v[5], v[6], v[7]);
-          };
-          // x is one piece per thread at most; the first of A's is loaded before it is waited for
-          const int r = tid / oct, c = tid % oct * 8;
-          float vx[8], va[8];
-          auto load_a = [&](int j, int ca) {  // zeros behind k_in
-            RawWeights8<WT> raw;
-            fetch_weights8(ad.a, (int64_t)j * bank.ka + kc + ca, raw);
-            weights8(raw, bank.wtype, va);
-          };
-          if (r < kSmallRows) load_row8(x + (int64_t)s_row[r] * a.ldx + kc + c, kn - c, x_vec != 0, vx);
-          if (r < ad.rank) load_a(r, c);
-          if (r < kSmallRows) put(r, c, vx);
-          if (r < ad.rank) put(kSmallRows + r, c, va);
-          for (int i = tid + kSmallThreads; i < ad.rank * oct; i += kSmallThreads) {
-            load_a(i / oct, i % oct * 8);
-            put(kSmallRows + i / oct, i % oct * 8, va);
-          }
-          __syncthreads();
-          const float* xr = s_x + (lane & 15) * kSmallLd;
+      for (int i = 0; i < RU; ++i) acc[i] = 0.0f;
+      for (int kc = k0; kc < k1; kc += kSmallChunk) {
+        const int kn = min(kSmallChunk, k1 - kc), oct = (kn + 7) / 8;
+        if (eighth != cta || kc > k0) __syncthreads();
+        auto put = [&](int r, int c, const float (&v)[8]) {
+          float4* d = reinterpret_cast<float4*>(s_x + r * kSmallLd + c);
+          d[0] = make_float4(v[0], v[1], v[2], v[3]);
+          d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        };
+        // x is one piece per thread at most; the first of A's is loaded before it is waited for
+        const int r = tid / oct, c = tid % oct * 8;
+        float vx[8], va[8];
+        auto load_a = [&](int j, int ca) {  // zeros behind k_in
+          RawWeights8<WT> raw;
+          fetch_weights8(ad.a, (int64_t)j * bank.ka + kc + ca, raw);
+          weights8(raw, bank.wtype, va);
+        };
+        if (r < kSmallRows) load_row8(x + (int64_t)s_row[r] * a.ldx + kc + c, kn - c, x_vec != 0, vx);
+        if (r < ad.rank) load_a(r, c);
+        if (r < kSmallRows) put(r, c, vx);
+        if (r < ad.rank) put(kSmallRows + r, c, va);
+        for (int i = tid + kSmallThreads; i < ad.rank * oct; i += kSmallThreads) {
+          load_a(i / oct, i % oct * 8);
+          put(kSmallRows + i / oct, i % oct * 8, va);
+        }
+        __syncthreads();
+        const float* xr = s_x + (lane & 15) * kSmallLd;
 #pragma unroll 4
-          for (int c = (lane >> 4) * 4; c < oct * 8; c += 8) {
-            const float4 v = *reinterpret_cast<const float4*>(xr + c);
+        for (int c = (lane >> 4) * 4; c < oct * 8; c += 8) {
+          const float4 v = *reinterpret_cast<const float4*>(xr + c);
 #pragma unroll
-            for (int i = 0; i < RU; ++i) {  // ranks there are not: the last one again
-              const float4 w4 = *reinterpret_cast<const float4*>(s_a + min(warp + i * kSmallWarps, ad.rank - 1) * kSmallLd + c);
-              acc[i] = fmaf(v.x, w4.x, fmaf(v.y, w4.y, fmaf(v.z, w4.z, fmaf(v.w, w4.w, acc[i]))));
-            }
+          for (int i = 0; i < RU; ++i) {  // ranks there are not: the last one again
+            const float4 w4 = *reinterpret_cast<const float4*>(s_a + min(warp + i * kSmallWarps, ad.rank - 1) * kSmallLd + c);
+            acc[i] = fmaf(v.x, w4.x, fmaf(v.y, w4.y, fmaf(v.z, w4.z, fmaf(v.w, w4.w, acc[i]))));
           }
         }
-        if (!started) cluster.barrier_wait();
-        started = true;
+      }
+      if (!started) cluster.barrier_wait();
+      started = true;
 #pragma unroll
-        for (int i = 0; i < RU; ++i) {
-          const int j = warp + i * kSmallWarps;
-          if (j >= ad.rank) break;
-          const float v = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 16));
-          // both halves of the lanes hold the sum: each sends it to half of the CTAs
-          float* mine = part + eighth * size + j * kSmallRows + (lane & 15);
-          for (int d = lane >> 4; d < ctas; d += 2) *cluster.map_shared_rank(mine, d) = v;
-        }
+      for (int i = 0; i < RU; ++i) {
+        const int j = warp + i * kSmallWarps;
+        if (j >= ad.rank) break;
+        const float v = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 16));
+        // both halves of the lanes hold the sum: each sends it to half of the CTAs
+        float* mine = part + eighth * size + j * kSmallRows + (lane & 15);
+        for (int d = lane >> 4; d < ctas; d += 2) *cluster.map_shared_rank(mine, d) = v;
       }
     }
-    if (ad.rank > 0) {
-      cluster.sync();
-      // The sets of partials take turns over the units that have this barrier: a set is written again only behind the
-      // next such unit's barrier, which every CTA reaches with its sums below done. (A unit of rank 0 must not count:
-      // the third unit's partials would land in a set that a slower CTA still sums.)
-      set ^= 1;
-      for (int i = tid; i < ad.rp * kSmallRows; i += kSmallThreads) {
-        float v = 0.0f;
-        if (i < size) {
+    cluster.sync();
+    // The sets of partials take turns over the units that have this barrier: a set is written again only behind the
+    // next such unit's barrier, which every CTA reaches with its sums below done. (A unit of rank 0 must not count:
+    // the third unit's partials would land in a set that a slower CTA still sums.)
+    set ^= 1;
+    for (int i = tid; i < ad.rp * kSmallRows; i += kSmallThreads) {
+      float v = 0.0f;
+      if (i < size) {
 #pragma unroll
-          for (int c = 0; c < kSmallParts; ++c) v = __fadd_rn(v, part[c * size + i]);
-          v = __fmul_rn(v, s_scale[i & 15]);
-        }
-        s_t[i] = v;  // zeros for the columns of B behind the rank
+        for (int c = 0; c < kSmallParts; ++c) v = __fadd_rn(v, part[c * size + i]);
+        v = __fmul_rn(v, s_scale[i & 15]);
       }
-      __syncthreads();
+      s_t[i] = v;  // zeros for the columns of B behind the rank
     }
+    __syncthreads();
     for (int item = tid; item < items; item += kSmallThreads) {
       if (item != tid) fetch(item);
       const int ch = n0 + item / 4 * 2;
@@ -329,9 +339,8 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
       for (int i = 0; i < 4; ++i) {
         if (q * 4 + i >= rows) break;
         YT* d = y + (int64_t)s_row[q * 4 + i] * a.ldy + ch;
-        // without a rank base as it is: adding a zero would change the sign of a zero and the bits of a NaN
-        d[0] = ad.rank > 0 ? from_f32<YT>(__fadd_rn(to_f32(b[0][i]), o[0][i])) : b[0][i];
-        if (ch + 1 < n1) d[1] = ad.rank > 0 ? from_f32<YT>(__fadd_rn(to_f32(b[1][i]), o[1][i])) : b[1][i];
+        d[0] = from_f32<YT>(__fadd_rn(to_f32(b[0][i]), o[0][i]));
+        if (ch + 1 < n1) d[1] = from_f32<YT>(__fadd_rn(to_f32(b[1][i]), o[1][i]));
       }
     }
   }
@@ -515,11 +524,12 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
   const int smem = small_smem_floats(bank.max_rank) * 4;
   // The function's limit is set to the same value whatever the bank (its largest rank's need): another thread may set
   // it between this call's setting and its launch.
-  constexpr int kMostRank = RU * kSmallWarps;
-  const cudaError_t e =
-      cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           small_smem_floats(kMostRank) * 4);
-  if (e != cudaSuccess) return e;
+  constexpr int kMost = small_smem_floats(RU * kSmallWarps) * 4;
+  if constexpr (kMost > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e != cudaSuccess) return e;
+  }
   // the largest clusters whose CTAs are all on the device at once (three per SM, two at ranks above 32; 132 SMs, since
   // a cluster of eight leaves some of a processing cluster's unused): 64 units of rank 16 took 20.5 us on clusters of
   // eight, in two waves, and take 13.1 us on clusters of four
