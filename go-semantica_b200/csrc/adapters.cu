@@ -530,11 +530,15 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
         cudaFuncSetAttribute(lowrank_small_kernel<XT, YT, WT, RU>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (e != cudaSuccess) return e;
   }
-  // the largest clusters whose CTAs are all on the device at once (three per SM, two at ranks above 32; 132 SMs, since
-  // a cluster of eight leaves some of a processing cluster's unused): 64 units of rank 16 took 20.5 us on clusters of
-  // eight, in two waves, and take 13.1 us on clusters of four
-  const int room = 132 * (RU <= 4 ? 3 : 2);
-  const int ctas = n_units <= room / 8 ? 8 : n_units <= room / 4 ? 4 : 2;
+  // The largest clusters that are all on the device at once. CTAs per SM: three, two at ranks above 32, one where their
+  // shared memory is above half of an SM's (ranks above 64). By these, 15, 33 or 48 clusters of eight run at once, and
+  // 33 per CTA and SM of four (a cluster leaves some of a processing cluster's SMs unused). One more unit, float32
+  // rows, 768 x 768, on eights in two waves / on fours: 49 of rank 16 13.3 / 10.7 us,
+  // 16 of rank 128 33.8 / 30.1, 33 of rank 128 50.7 / 31.0. One less on eights: 48 of rank 16 8.6, 33 of rank 64 16.1,
+  // 15 of rank 128 18.0 us.
+  constexpr int kEights[3] = {15, 33, 48};
+  const int fit = 227 * 1024 / (smem + 1024), most = RU <= 4 ? 3 : 2, per_sm = fit < most ? fit : most;
+  const int ctas = n_units <= kEights[per_sm - 1] ? 8 : n_units <= 33 * per_sm ? 4 : 2;
   const int clusters = n_units < 2048 ? n_units : 2048;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(clusters * ctas));
