@@ -28,6 +28,12 @@ int same_device(const sem_context* a, const sem_context* b) {
   return set_error(SEM_EINVAL, "the plan is on device %d, the operator on device %d", b->device, a->device);
 }
 
+// Holds a context's lock while a call enqueues on the context's own stream: the model's forward may be capturing that
+// stream on another thread, and would take the call into its graph. (Taken before a plan's lock.)
+std::unique_lock<std::mutex> own_stream(sem_context* ctx, cudaStream_t st) {
+  return st == ctx->stream ? std::unique_lock<std::mutex>(ctx->mu) : std::unique_lock<std::mutex>();
+}
+
 int capturing(cudaStream_t st, bool* out) {
   cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
   SEM_CUDA(cudaStreamIsCapturing(st, &s));
@@ -215,6 +221,7 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, LowRankArgs args, con
   if (int rc = same_device(w->ctx, plan->ctx)) return rc;
   DeviceGuard dg(w->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : w->ctx->stream;
+  const auto own = own_stream(w->ctx, st);
   std::lock_guard<std::mutex> lk(plan->mu);
   if (plan->max_adapter >= w->bank.n_adapters)
     return set_error(SEM_EINVAL, "low-rank adapters: the plan uses adapter %d, the bank has %d", plan->max_adapter,
@@ -391,6 +398,7 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
     return set_error(SEM_EINVAL, "block norm: one buffer with two row strides");
   DeviceGuard dg(b->ctx->device);
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : b->ctx->stream;
+  const auto own = own_stream(b->ctx, st);
   std::unique_lock<std::mutex> lk;  // until the call is enqueued, as in lowrank_launch
   if (plan) {
     if ((rc = same_device(b->ctx, plan->ctx))) return rc;
@@ -416,11 +424,13 @@ int block_norm_run(sem_block_norm* b, sem_adapter_plan* plan, int64_t rows, cons
   return SEM_OK;
 }
 
-// Frees a handle once the work enqueued on its device is done.
+// Frees a handle once the work enqueued on its device is done (not while the context's stream is captured: a device
+// with a captured stream cannot be waited for).
 template <class T>
 int free_handle(T* h) {
   if (!h) return SEM_OK;
   DeviceGuard dg(h->ctx->device);
+  std::lock_guard<std::mutex> lk(h->ctx->mu);
   cudaDeviceSynchronize();
   delete h;
   return SEM_OK;
@@ -436,15 +446,19 @@ sem_adapter_plan::~sem_adapter_plan() {
 extern "C" {
 
 int sem_adapter_plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapter_plan** out) {
-  return sem::guarded([&]() -> int { return sem::plan_create(ctx, max_rows, max_seqs, out); });
+  return sem::guarded([&]() -> int {
+    const auto own = ctx ? sem::own_stream(ctx, ctx->stream) : std::unique_lock<std::mutex>();
+    return sem::plan_create(ctx, max_rows, max_seqs, out);
+  });
 }
 
 int sem_adapter_plan_set(sem_adapter_plan* plan, const int32_t* offsets, const int32_t* adapters, int32_t n_seqs,
                          void* stream) {
   return sem::guarded([&]() -> int {
     if (!plan) return sem::set_error(SEM_EINVAL, "null argument");
-    return sem::plan_set(plan, offsets, adapters, n_seqs,
-                         stream ? static_cast<cudaStream_t>(stream) : plan->ctx->stream);
+    cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : plan->ctx->stream;
+    const auto own = sem::own_stream(plan->ctx, st);
+    return sem::plan_set(plan, offsets, adapters, n_seqs, st);
   });
 }
 

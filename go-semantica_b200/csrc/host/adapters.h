@@ -36,6 +36,7 @@ namespace sem {
 
 constexpr int32_t kLowRankMaxDim = 65536;
 
+// plan_create enqueues on the context's stream, plan_set on `st`: the caller holds the context's lock where that is it.
 int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapter_plan** out);
 int plan_set(sem_adapter_plan* p, const int32_t* offsets, const int32_t* adapters, int32_t n_seqs, cudaStream_t st);
 AdapterPlanDev plan_device(const sem_adapter_plan* p);

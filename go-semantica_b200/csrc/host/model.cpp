@@ -1501,6 +1501,7 @@ int sem_model_adapters_free(sem_model_adapters* a) {
   return sem::guarded([&]() -> int {
     if (!a) return SEM_OK;
     sem::DeviceGuard dg(a->model->ctx->device);
+    std::lock_guard<std::mutex> lk(a->model->ctx->mu);  // not while a forward on another thread captures the stream
     cudaStreamSynchronize(a->model->ctx->stream);
     delete a;
     return SEM_OK;

@@ -297,7 +297,8 @@ int sem_q8_gemm_noalloc(sem_q8_weight *w, const float *d_a, int32_t m, float *d_
  * pointers, are enqueued on `stream` (NULL = the handle's context stream) and
  * return without synchronising. They allocate nothing and keep no state, so
  * calls may overlap, on one stream or several, and may be captured into CUDA
- * graphs.
+ * graphs. On the context's own stream they take their turn with the context's
+ * other calls (sem_embed keeps it until its outputs are there).
  * ---------------------------------------------------------------------- */
 
 /* Element types of the operators' rows and weights. */

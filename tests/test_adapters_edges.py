@@ -11,6 +11,7 @@ import pytest
 
 from conftest import ROOT
 from test_adapters import BUILD, DT, LowRankCase, _batch, path  # noqa: F401 (a fixture)
+from test_model_adapters import model, tensors  # noqa: F401 (fixtures)
 
 
 def _threads(*work):
@@ -371,4 +372,64 @@ def test_a_nan_of_any_payload_stays_one(ctx, path):
     want, bound = c.oracle()
     rest = [i for i in range(73) if i not in bad]
     assert ((got[rest].double() - want[rest]).abs() <= bound[rest]).all()
+    c.close()
+
+
+@pytest.mark.gpu
+def test_calls_on_the_contexts_stream_beside_captured_forwards(ctx, model, tensors):
+    # One thread embeds batches of new shapes, whose forwards are captured on the context's stream; another makes
+    # plans and calls operators there. Neither may end in the other's capture.
+    import torch
+    import adapters as ad
+    import synth
+    shapes = [[5 + i, 9, 30 + 2 * i] for i in range(60)]
+    batches = [synth.token_batch(i, s, 64) for i, s in enumerate(shapes)]
+    want = [model.forward_batch(*b) for b in batches[:4]]
+    c = LowRankCase(ctx, [40, 3], [0, -1], [16], 96, 160)
+    bn = ad.BlockNorm(ctx, 96, 1e-6, np.ones(96, np.float32), np.ones(96, np.float32))
+    o, h = torch.randn(43, 96, device="cuda"), torch.randn(43, 96, device="cuda")
+    ho, y = torch.empty_like(h), torch.empty_like(o)
+    torch.cuda.synchronize()
+    bn.run(43, o.data_ptr(), 0, h.data_ptr(), 0, ho.data_ptr(), y.data_ptr(), c.plan)
+    c.bank.check()
+    ho1, y1 = ho.clone(), y.clone()
+    torch.cuda.synchronize()
+    done, rounds, got = threading.Event(), [0], [None] * len(batches)
+
+    def embed():
+        try:
+            for i, b in enumerate(batches):
+                got[i] = model.forward_batch(*b)
+        finally:
+            done.set()
+
+    def operators():
+        while not done.is_set() or rounds[0] < 5:
+            plan = ad.AdapterPlan(ctx, c.rows, 2)
+            plan.set(c.offs, c.use)
+            c.bank.apply(plan, c.dx.data_ptr(), 0, c.dy.data_ptr(), 0, c.dbase.data_ptr())
+            bn.run(43, o.data_ptr(), 0, h.data_ptr(), 0, ho.data_ptr(), y.data_ptr(), plan)
+            c.bank.check()
+            c.verify(c.dy)
+            assert torch.equal(ho, ho1) and torch.equal(y, y1)
+            for t in (c.dy, ho, y):
+                t.fill_(77)
+            torch.cuda.current_stream().synchronize()
+            plan.close()
+            model.load_adapters([]).close()
+            rounds[0] += 1
+
+    _threads(embed, operators)
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            np.testing.assert_array_equal(a, b)
+    c.dy.fill_(77)
+    torch.cuda.synchronize()
+    # the captured forwards hold nothing of the other thread's: replayed, they leave y alone
+    for i, b in enumerate(batches[-8:]):
+        for a, w in zip(model.forward_batch(*b), got[len(batches) - 8 + i]):
+            np.testing.assert_array_equal(a, w)
+    torch.cuda.synchronize()
+    assert (c.dy == 77).all()
+    bn.close()
     c.close()
