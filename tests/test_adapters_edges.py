@@ -433,3 +433,45 @@ def test_calls_on_the_contexts_stream_beside_captured_forwards(ctx, model, tenso
     assert (c.dy == 77).all()
     bn.close()
     c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,w,k", [("f32", "f32", 768), ("f16", "bf16", 768), ("bf16", "bf16", 517)])
+def test_a_sequence_alone_and_in_other_batches(ctx, path, x, w, k):
+    # With one kernel for both, a sequence's rows have the same bits alone, in a small batch and in a large one. AUTO
+    # takes the kernel that suits the whole batch: there the two are each within the bound of the operator.
+    import torch
+    lengths, use, ranks = [300, 20, 7, 150], [0, 1, 2, 1], [16, 24, 100]
+    c = LowRankCase(ctx, lengths, use, ranks, k, 256, x=x, w=w)
+    c.run(ctx)
+    together, offs = c.dy.clone(), c.offs
+    want, bound = c.oracle()
+
+    def check(got, at):
+        if path == "auto":
+            assert ((got.cpu().double() - want[at]).abs() <= bound[at]).all()
+        else:
+            assert torch.equal(got, together[at])
+
+    dx, dbase = c.dx, c.dbase
+    for s, a in enumerate(use):
+        at = slice(int(offs[s]), int(offs[s + 1]))
+        c.plan.set([0, lengths[s]], [a])
+        c.dx, c.dbase, c.dy = dx[at].clone(), dbase[at].clone(), torch.full_like(together[at], 77)
+        torch.cuda.synchronize()
+        c.call(ctx.stream)
+        c.bank.check()
+        check(c.dy, at)
+    # behind 6000 other rows, in a plan with room for them
+    import adapters as ad
+    big = ad.AdapterPlan(ctx, 6000 + c.rows, 8)
+    big.set(np.concatenate([[0], 6000 + offs]), [2] + use)
+    c.plan.close()
+    c.plan = big
+    c.dx, c.dbase = torch.cat([dx[:1].expand(6000, -1), dx]), torch.cat([dbase[:1].expand(6000, -1), dbase])
+    c.dy = torch.full_like(c.dbase, 77)
+    torch.cuda.synchronize()
+    c.call(ctx.stream)
+    c.bank.check()
+    check(c.dy[6000:], slice(None))
+    c.close()
