@@ -120,9 +120,12 @@ __device__ __forceinline__ void weights8(const RawWeights8<WT>& r, int wtype, fl
 // latency. The shares do not go by the batch (a row's sums are the same for
 // any cluster size: the input channels are cut in eight, and a CTA of a
 // smaller cluster sums several of the eight one after the other). Float32 FMA
-// throughout. Bound by that latency (device time): 12 float32 rows, 768 x 768,
-// rank 8, 4 us; 48 sequences of 1 to 24 fp16 rows, each with an adapter of its
-// own, 768 x 1280, rank to 16, 13 us.
+// throughout. Bound by that latency (per call of a CUDA graph): 12 float32 rows,
+// 768 x 768, rank 8, 5.5 us. One fp16 unit of rank 16 takes 6.3 us at 768 x 256,
+// 7.4 at 768 x 1280, 8.6 at 768 x 2304 (a thread's second and third round of
+// output channels wait for base and B), 48 at once 7.9, 10.0 and 12.3. 48
+// sequences of 1 to 24 fp16 rows, each with an adapter of its own, 768 x 1280,
+// rank to 16, 12.9 us: 63 units, more than clusters of eight fit.
 constexpr int kSmallParts = 8, kSmallThreads = 256, kSmallWarps = kSmallThreads / 32;
 constexpr int kSmallChunk = 128, kSmallLd = kSmallChunk + 4;  // input channels staged at a time, padded (banks)
 constexpr int kSmallRows = kAdapterSmallRows;
@@ -354,9 +357,10 @@ __global__ void __launch_bounds__(kSmallThreads, RU <= 4 ? 3 : 2)
 // TPR threads hold one row in registers, NC chunks of VEC elements each, so o
 // and h are read once and h_out and y written once; the two sums of squares
 // are float32 partial sums joined by a fixed tree. Bound by HBM: 131072 float32
-// rows of 768 take 242 us, the rate of a plain copy. Rows without alignment go
-// by single elements: 10599 rows of 1153, fp16 over a float32 residual, 31 us
-// (18.6 at the copy's rate).
+// rows of 768 take 240 us, the rate of a plain copy; fp16 or bf16 rows over a
+// float32 residual 191 us (184 at that rate), over a 16-bit one 155 us (123).
+// Rows without alignment go by single elements: 10599 rows of 1153, fp16 over a
+// float32 residual, 32 us (18.6 at the copy's rate).
 constexpr int kNormThreads = 128;
 
 template <int TPR>

@@ -53,7 +53,8 @@ int plan_create(sem_context* ctx, int64_t max_rows, int32_t max_seqs, sem_adapte
   p->max_rows = max_rows;
   p->max_seqs = max_seqs;
   const int64_t large = adapter_plan_max_large(max_rows, max_seqs);
-  // one upload: counts, sequences (pos, row0, seq, adapter), tiles
+  // one buffer: counts and sequences (pos, row0, seq, adapter), large tiles, small tiles; what a batch fills of the three
+  // goes up in a copy each
   p->up_bytes = 16 + (size_t)round_up((size_t)4 * max_seqs + 4, 4) * 4 + ((size_t)large + max_seqs + 1) * sizeof(AdapterTile);
   cudaError_t e = p->up.ensure(p->up_bytes);
   if (e == cudaSuccess) e = p->maps.ensure((size_t)3 * (max_rows > 0 ? max_rows : 1) * 4);
@@ -239,11 +240,12 @@ int lowrank_launch(sem_lowrank* w, sem_adapter_plan* plan, LowRankArgs args, con
 
 // Up to this many multiply-adds a call runs on the CUDA cores as a whole: the
 // tensor-core kernel's pipeline takes longer to fill than they take. Measured
-// (CUDA cores / tensor cores, 768 x 768, rank 16): INT8 codes 12.6 M 8.3 / 12.0
-// us, 25 M 12.1 / 13.2, 50 M 18.7 / 14.5; float32 rows, whose conversion the
-// tensor cores wait for, 25 M 11.4 / 19.6, 63 M 21.7 / 21.8; 517 x 1001, 212 M
-// 43.1 / 34.6. A tile of up to 16 rows counts as eight (256 single fp16 rows of
-// as many adapters: 33.3 / 25.0 us; 64 tiles of 12 rows: 13.1 on the CUDA cores).
+// (CUDA cores / tensor cores, 768 x 768, rank 16, per call of a CUDA graph):
+// INT8 codes 12.6 M 7.8 / 12.0 us, 25 M 11.5 / 13.5, 50 M 18.2 / 14.8; float32
+// rows, whose conversion the tensor cores wait for, 25 M 11.0 / 20.2, 63 M
+// 21.3 / 21.9; 517 x 1001, 212 M 43.2 / 34.9. A tile of up to 16 rows counts as
+// eight (256 single fp16 rows of as many adapters: 32.1 / 26.7 us; 64 tiles of 12
+// rows: 11.1 / 15.7).
 constexpr int64_t kLowRankSmallWork = 28000000, kLowRankSmallWorkF32 = 60000000;
 
 // One launch for all tiles of the plan, also for an empty plan when it is

@@ -9,15 +9,17 @@
 // along the channels of a row, coalesced. Two expand accumulators hold the
 // even and the odd channels of 256: a thread owns two neighbours.
 //
-// Numbers. No operand loses bits that count: every value goes in as the parts
-// that give at least 21 bits, and the products of parts (all but those below
-// 2^-22) are accumulated in float32 in TMEM. Shrink of float32 rows: tf32 (11
+// Numbers. Every value goes in as the parts that give at least 21 bits (22 of a
+// float32's 24), and the products of parts (all but those below 2^-22) are
+// accumulated in float32 in TMEM. Shrink of float32 rows: tf32 (11
 // bits), x and float32 weights as hi + lo. Shrink of 16-bit rows (and INT8
 // codes held as fp16): kind::f16 on the rows as they are, A in x's type: one
 // part where the types are the same, else two bf16 parts of fp16, three bf16
 // parts of float32, or two fp16 parts of a rank's weights scaled by a power of
-// two (undone in t). Expand: tf32, t as hi + lo, B as stored or hi + lo. Only
-// y's own rounding loses bits.
+// two (undone in t). Expand: tf32, t as hi + lo, B as stored or hi + lo. The
+// tensor core cuts its sums instead of rounding them, which is most of the error:
+// float32 rows of 768 values, rank 4 to 104, 1.1e-7 to 2.9e-7 of y's size, where
+// float32 products and sums with rounding (the CUDA-core kernel) are 4e-8 off.
 //
 // Bound by HBM at the ranks in use: a row moves k |x| + 2 n |y| bytes and
 // needs 2 r (k + n) flops (r = 16, 768 x 768, float32: 9.2 KB against 49
@@ -36,9 +38,9 @@
 //     ahead of the accumulators and across units.
 // One persistent CTA per SM. Per call (device time; bytes at 6.56 TB/s, the
 // rate of a plain copy, in parentheses):
-//   65536 float32 rows, 768 x 768, rank 16:             115 us (92)
-//   196608 rows of codes, 1152 x 768, rank 32:          290 us (253)
-//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    292 us (181)
+//   65536 float32 rows, 768 x 768, rank 16:             113 us (92)
+//   196608 rows of codes, 1152 x 768, rank 32:          280 to 300 us (253)
+//   110213 ragged bf16 rows, 768 x 2304, rank to 64:    287 us (181)
 //   16384 fp16 rows, 768 x 1280, rank 128, f32 weights:  93 us (17)
 //   6075 ragged float32 rows, 517 x 1001, rank to 23:    35 us (9)
 // The first two are near the copy's rate. In the third a unit reads 0.6 MB of
