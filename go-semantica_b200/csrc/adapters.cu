@@ -535,7 +535,7 @@ cudaError_t small_ranks(const LowRankBank& bank, const AdapterPlanDev& plan, int
     if (e != cudaSuccess) return e;
   }
   // The largest clusters that are all on the device at once. CTAs per SM: three, two at ranks above 32, one where their
-  // shared memory is above half of an SM's (ranks above 64). By these, 15, 33 or 48 clusters of eight run at once, and
+  // shared memory is above half of an SM's (ranks above 65). By these, 15, 33 or 48 clusters of eight run at once, and
   // 33 per CTA and SM of four (a cluster leaves some of a processing cluster's SMs unused). One more unit, float32
   // rows, 768 x 768, on eights in two waves / on fours: 49 of rank 16 13.3 / 10.7 us,
   // 16 of rank 128 33.8 / 30.1, 33 of rank 128 50.7 / 31.0. One less on eights: 48 of rank 16 8.6, 33 of rank 64 16.1,
